@@ -27,7 +27,8 @@
  * is written (the fills the reference did in Python / THCudaTensor_zero are
  * part of the op), so callers may pass uninitialised memory.
  *
- * All data is fp32 (GENRE_F32) except nndistance indices (GENRE_I32).
+ * All data is fp32 (GENRE_F32) except nndistance indices (GENRE_I32) and what the group normalisation and the gradient ops at
+ * the end of this file say of theirs.
  */
 #ifndef GENRE_HIP_H
 #define GENRE_HIP_H
@@ -41,13 +42,13 @@ extern "C" {
 #define GENRE_ABI_VERSION 5
 #define GENRE_MAX_DIMS 5
 
-enum { GENRE_F32 = 0, GENRE_I32 = 1 };
+enum { GENRE_F32 = 0, GENRE_I32 = 1, GENRE_BF16 = 2, GENRE_F16 = 3, GENRE_F64 = 4 };
 
 /* Tensor view: device pointer, sizes and ELEMENT strides (not bytes). */
 typedef struct genre_tensor {
     void   *data;
     int32_t ndim;
-    int32_t dtype;                   /* GENRE_F32 | GENRE_I32 */
+    int32_t dtype;                   /* GENRE_F32 | ... (one of the enum above) */
     int64_t size[GENRE_MAX_DIMS];
     int64_t stride[GENRE_MAX_DIMS];
 } genre_tensor;
@@ -443,6 +444,53 @@ int genre_render_bm_backward(const genre_tensor *grad_out, const genre_tensor *g
                              const genre_tensor *depth_weight, const genre_tensor *ps_scratch,
                              const genre_tensor *tr_scratch, const genre_tensor *p_stash, const genre_tensor *mask,
                              float pre_scale, int pull_brick, void *stream);
+
+/* ---- training-step ops (no counterpart in the reference: its networks normalise over the batch, networks/networks.py:147-190,
+ * and its optimiser steps on the gradients as they come, train.py:137-214) ---------------------------------------- */
+
+/* Group normalisation with its activation.  x, y, dy, dx: [N,C,S], S the product of the spatial sizes (1 for none), all fp32,
+ * all bf16 or all fp16, and all channels last (stride[1] == 1, one row of C values per position, rows may have gaps) or all
+ * channels first (stride[2] == 1, gaps between the planes allowed); image strides are free, no pointer needs more alignment
+ * than its type's.  groups divides C.  weight, bias (and dw, db): [C] contiguous, each of the three types, or NULL (weight 1,
+ * bias 0; gradient not wanted).  act: 0 none, 1 ReLU, 2 leaky ReLU (`slope` below zero; only act 2 reads it), 3 SiLU.
+ *   forward:  y = act((x - mean) / sqrt(var + eps) * weight + bias), mean and biased variance of each image and group;
+ *             stats fp64 [2,N,groups] receives mean and 1 / sqrt(var + eps)
+ *   backward: from x, dy and the forward's stats; dx (NULL: not wanted), dw, db
+ * ws: fp64 scratch of at least genre_group_norm_workspace(x, groups, backward) values (-1: refused), undefined before and after;
+ * two calls that may run at once need two.  Sums and statistics are fp64 and added in a fixed order: equal inputs, equal bits.
+ * The derivative of (leaky) ReLU at 0 is that of the negative side.  N or S of zero: nothing but dw = db = 0 is written. */
+int64_t genre_group_norm_workspace(const genre_tensor *x, int groups, int backward);
+
+int genre_group_norm_forward(const genre_tensor *x, const genre_tensor *y, const genre_tensor *weight, const genre_tensor *bias,
+                             const genre_tensor *stats, const genre_tensor *ws, int groups, double eps, int act, float slope,
+                             void *stream);
+
+int genre_group_norm_backward(const genre_tensor *x, const genre_tensor *dy, const genre_tensor *weight,
+                              const genre_tensor *bias, const genre_tensor *stats, const genre_tensor *dx,
+                              const genre_tensor *dw, const genre_tensor *db, const genre_tensor *ws, int groups, int act,
+                              float slope, void *stream);
+
+/* Many tensors at once.  ptrs[i], numels[i] (may be 0), dtypes[i] (GENRE_F32 | GENRE_BF16 | GENRE_F16), i < n: host arrays, read
+ * before the call returns; the tensors' values lie without gaps from ptrs[i] on, with no more alignment than their type's, and
+ * no two tensors overlap where one is written.
+ *   genre_grad_norm: out fp32 [2] = the norm of all values together -- norm_type 2: sqrt of the sum of squares (fp64 sums);
+ *     0: the largest magnitude (NaN if one is) -- and the factor min(1, max_norm / (norm + 1e-6)) (NaN stays NaN; 1 for
+ *     max_norm = infinity).  ws: fp64 scratch of at least genre_grad_workspace(numels, n) values.
+ *   genre_grad_scale: every value times factor[0] (fp32, on the device), rounded to its type; 1 leaves the memory untouched
+ *   genre_adam_step: with g' = g factor[0] + weight_decay p (factor NULL: 1; decoupled != 0: p is scaled by 1 - lr weight_decay
+ *     instead),  m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2,
+ *     p -= lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps);  p and g of dtypes[i], m and v fp32; g is not written. */
+int64_t genre_grad_workspace(const int64_t *numels, int n);
+
+int genre_grad_norm(const void *const *ptrs, const int64_t *numels, const int32_t *dtypes, int n, int norm_type, float max_norm,
+                    const genre_tensor *out, const genre_tensor *ws, void *stream);
+
+int genre_grad_scale(void *const *ptrs, const int64_t *numels, const int32_t *dtypes, int n, const genre_tensor *factor,
+                     void *stream);
+
+int genre_adam_step(void *const *p, const void *const *g, void *const *m, void *const *v, const int64_t *numels,
+                    const int32_t *dtypes, int n, const genre_tensor *factor, int64_t step, double lr, double beta1,
+                    double beta2, double eps, double weight_decay, int decoupled, void *stream);
 
 #ifdef __cplusplus
 }
