@@ -26,7 +26,7 @@ from .toolbox.calc_prob.calc_prob.functions.calc_prob import CalcStopProb
 from .toolbox.spherical_proj import render_spherical, sph_pad, gen_sph_grid
 from .toolbox.nndistance.functions.nnd import (NNDFunction, nndistance, nndistance_w_idx, nndistance_score)
 from .toolbox.nndistance.modules.nnd import NNDModule
-from .toolbox.group_norm.functions.group_norm import GroupNormActFunction, group_norm_act
+from .toolbox.group_norm.functions.group_norm import group_norm_act
 from .toolbox.group_norm.modules.group_norm import GroupNormAct
 from .toolbox.grad_clip.functions.grad_clip import grad_norm, clip_grads_, clip_grad_norm_, clip_adam_step_
 
@@ -34,5 +34,4 @@ __all__ = ["CameraBackProjection", "SphericalBackProjection", "get_surface_mask"
            "Camera_back_projection_layer", "CalcStopProb", "render_spherical", "sph_pad",
            "gen_sph_grid", "NNDFunction", "nndistance", "nndistance_w_idx", "nndistance_score",
            "NNDModule",
-           "GroupNormActFunction", "group_norm_act", "GroupNormAct", "grad_norm", "clip_grads_", "clip_grad_norm_",
-           "clip_adam_step_"]
+           "group_norm_act", "GroupNormAct", "grad_norm", "clip_grads_", "clip_grad_norm_", "clip_adam_step_"]

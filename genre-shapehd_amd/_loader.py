@@ -1,6 +1,7 @@
 """ctypes binding of libgenre_hip.so (the C ABI declared in include/genre_hip.h).
 
-This is the only place the Python host side touches native code.  There is NO
+This is the only place the Python host side touches native code (the training-step ops go
+through a PyTorch extension over the same library, loaded here too).  There is NO
 CPU fallback: if the library is missing (not built) the import fails loudly,
 and every op refuses non-CUDA tensors.  The three objects exported at the
 bottom -- ``cam_bp_lib``, ``calc_prob_lib``, ``my_lib`` -- carry the same
@@ -9,19 +10,18 @@ function names and argument orders as the reference's cffi modules
 my_lib_cuda.h:1-4), so the autograd Functions read like the reference's.
 """
 import ctypes as C
+import importlib.util
 import os
-from array import array
 
 import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # (GENRE_HIP_LIB: an A/B variant of the library, tools/build_variants.sh -- measurement only; the default is the in-tree build)
 LIB_PATH = os.environ.get("GENRE_HIP_LIB") or os.path.join(_HERE, "csrc", "libgenre_hip.so")
+BINDING_PATH = os.path.join(_HERE, "csrc", "genre_torch.so")
 ABI_VERSION = 5
 _MAX_DIMS = 5
 _F32, _I32 = 0, 1
-_BF16, _F16, _F64 = 2, 3, 4
-_FLOATS = {torch.float32: _F32, torch.bfloat16: _BF16, torch.float16: _F16}
 
 
 class GenreTensor(C.Structure):
@@ -71,18 +71,6 @@ def _load():
     lib.genre_cam_forward_plan.argtypes = [T, T, C.c_float, C.c_float]
     lib.genre_cam_forward_plan.restype = C.c_int
     lib.genre_cam_cell.restype = C.c_int
-    I, D, F = C.c_int, C.c_double, C.c_float
-    for name, argtypes in (("genre_group_norm_forward", [T] * 6 + [I, D, I, F, V]),
-                           ("genre_group_norm_backward", [T] * 9 + [I, I, F, V]),
-                           ("genre_grad_norm", [V, V, V, I, I, F, T, T, V]),
-                           ("genre_grad_scale", [V, V, V, I, T, V]),
-                           ("genre_adam_step", [V] * 6 + [I, T, C.c_int64] + [D] * 5 + [I, V]),
-                           ("genre_group_norm_workspace", [T, I, I]), ("genre_grad_workspace", [V, I])):
-        fn = getattr(lib, name, None)
-        if fn is None:
-            raise ImportError("libgenre_hip.so does not export %s -- rebuild (make -C genre-shapehd_amd/csrc)" % name)
-        fn.argtypes = argtypes
-        fn.restype = C.c_int64 if name.endswith("_workspace") else I
     return lib
 
 
@@ -326,90 +314,23 @@ class _GlueLib:
                      scalars=(C.c_float(scale_25d),), out=(3,))
 
 
-def _enqueue(name, dev, *args):
-    """`name`(args..., stream) on torch's current stream of `dev`; raise on failure"""
-    if dev.index == torch.cuda.current_device():
-        ok = getattr(_lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
-    else:
-        with torch.cuda.device(dev):
-            ok = getattr(_lib, name)(*args, torch.cuda.current_stream(dev).cuda_stream)
-    if ok != 1:
-        raise RuntimeError("%s failed: %s" % (name, _lib.genre_last_error().decode()))
+class _TrainingLib:
+    """the training-step ops (group normalisation, gradient norm, clipping, Adam step; extension).  They are reached through
+    csrc/genre_torch.so, a PyTorch extension over the same C ABI: their calls are many and short, or carry hundreds of tensors,
+    and ctypes would take longer than the kernels.  Loaded at the first use and bound to this module's library."""
 
-
-def _flat(t, dtype=_F32):
-    n = t.numel()
-    return GenreTensor(t.data_ptr(), 1, dtype, (n,), (1,))
-
-
-class _GroupNormLib:
-    """group normalisation with its activation (extension).  Maps come as (tensor, strides) with the element strides of image,
-    channel and position; weight, bias, dw, db: [C] contiguous tensors or None"""
-
-    ACTS = {"none": 0, "relu": 1, "leaky_relu": 2, "silu": 3}
-
-    @staticmethod
-    def _map(t, shape, strides):
-        return GenreTensor(t.data_ptr(), 3, _FLOATS[t.dtype], shape, strides)
-
-    @staticmethod
-    def _param(t):
-        return None if t is None else _flat(t, _FLOATS[t.dtype])
-
-    @classmethod
-    def _scratch(cls, desc, groups, backward, dev):
-        need = _lib.genre_group_norm_workspace(desc, groups, backward)
-        if need < 0:
-            raise RuntimeError("group norm: %s" % _lib.genre_last_error().decode())
-        return torch.empty(need, dtype=torch.float64, device=dev)
-
-    @classmethod
-    def forward(cls, x, xs, y, ys, shape, weight, bias, stats, groups, eps, act, slope):
-        dx = cls._map(x, shape, xs)
-        ws = cls._scratch(dx, groups, 0, x.device)
-        _enqueue("genre_group_norm_forward", x.device, dx, cls._map(y, shape, ys), cls._param(weight), cls._param(bias), _flat(stats, _F64),
-                 _flat(ws, _F64), groups, eps, act, slope)
-
-    @classmethod
-    def backward(cls, x, xs, dy, dys, shape, weight, bias, stats, dx, dxs, dw, db, groups, act, slope):
-        d = cls._map(x, shape, xs)
-        ws = cls._scratch(d, groups, 1, x.device)
-        _enqueue("genre_group_norm_backward", x.device, d, cls._map(dy, shape, dys), cls._param(weight), cls._param(bias), _flat(stats, _F64),
-                 None if dx is None else cls._map(dx, shape, dxs), cls._param(dw), cls._param(db), _flat(ws, _F64), groups, act, slope)
-
-
-class _Many:
-    """the host arrays that the ops over many tensors read: addresses of each list, sizes and types"""
-
-    def __init__(self, first, *more):
-        dev = first[0].device
-        types = [_FLOATS.get(t.dtype, -1) for t in first]
-        if -1 in types:
-            raise RuntimeError("dtype %s not supported (fp32, bf16 or fp16)" % first[types.index(-1)].dtype)
-        self.n, self.device = len(first), dev
-        self._keep = [array("q", map(torch.Tensor.data_ptr, ts)) for ts in (first, *more)]
-        self._keep += [array("q", map(torch.Tensor.numel, first)), array("i", types)]
-        self.lists = [a.buffer_info()[0] for a in self._keep[:-2]]
-        self.numels, self.types = (a.buffer_info()[0] for a in self._keep[-2:])
-
-
-class _GradLib:
-    """ops over many tensors at once (extension): norm, scaling, Adam step.  The lists hold gap-free tensors of one device"""
-
-    @staticmethod
-    def norm(many, norm_type, max_norm, out):
-        need = _lib.genre_grad_workspace(many.numels, many.n)
-        ws = torch.empty(need, dtype=torch.float64, device=many.device)
-        _enqueue("genre_grad_norm", many.device, many.lists[0], many.numels, many.types, many.n, norm_type, max_norm, _flat(out), _flat(ws, _F64))
-
-    @staticmethod
-    def scale(many, factor):
-        _enqueue("genre_grad_scale", many.device, many.lists[0], many.numels, many.types, many.n, _flat(factor))
-
-    @staticmethod
-    def adam(many, factor, step, lr, beta1, beta2, eps, weight_decay, decoupled):
-        _enqueue("genre_adam_step", many.device, *many.lists, many.numels, many.types, many.n, None if factor is None else _flat(factor), step,
-                 lr, beta1, beta2, eps, weight_decay, 1 if decoupled else 0)
+    def __getattr__(self, name):
+        if not os.path.exists(BINDING_PATH):
+            raise ImportError("genre-shapehd_amd: %s is not built. Run `make -C genre-shapehd_amd/csrc`" % BINDING_PATH)
+        spec = importlib.util.spec_from_file_location("genre_torch", BINDING_PATH)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+        mod.bind_library(LIB_PATH)
+        for fn in ("group_norm_act", "grad_norm", "clip_grads", "adam_step"):
+            self.__dict__[fn] = getattr(mod, fn)
+        if name not in self.__dict__:
+            raise AttributeError(name)
+        return self.__dict__[name]
 
 
 class _MyLib:
@@ -440,6 +361,4 @@ calc_prob_lib = _CalcProbLib()
 my_lib = _MyLib()
 render_lib = _RenderLib()
 glue_lib = _GlueLib()
-group_norm_lib = _GroupNormLib()
-grad_lib = _GradLib()
-Many = _Many
+training_lib = _TrainingLib()

@@ -1,8 +1,5 @@
-"""Stands in for the reference's cffi extension package `_ext` (built there by
-torch.utils.ffi, toolbox/*/build.py): re-exports the ctypes shim object(s) of
-genre-shapehd_amd/_loader.py under the reference's names.  The loader is located from this
-file's own path and shared process-wide, so the reference's import lines work whether this
-tree is imported as `genre_shapehd_amd.toolbox...`, as `toolbox...` or as `nndistance...`."""
+"""The native ops behind this package: the object of genre-shapehd_amd/_loader.py, located from this file's own path and shared
+process-wide, so that it is the same one whether this tree is imported as `genre_shapehd_amd.toolbox...` or as `toolbox...`."""
 import importlib.util
 import os
 import sys
@@ -26,5 +23,4 @@ def _loader():
     return mod
 
 
-grad_lib = _loader().grad_lib
-Many = _loader().Many
+training_lib = _loader().training_lib
