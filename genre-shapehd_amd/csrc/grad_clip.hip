@@ -46,49 +46,62 @@ __device__ __forceinline__ Share share(const Table<P> &t, unsigned block)
     return {k, lo, lo + t.chunk < n ? lo + t.chunk : n};
 }
 
-template <class T, int V>
+// V values; no alignment beyond the type's is asked for (gfx950 loads and stores 16 bytes at any address)
+template <class R, int V> using vec = R __attribute__((ext_vector_type(V), aligned(sizeof(R))));
+template <class T, int V, bool STREAM = false>
 __device__ __forceinline__ void load(const typename T::raw *p, float (&v)[V])
 {
-    typename T::raw t[V];
-    __builtin_memcpy(t, p, sizeof(t));                                     // (no alignment beyond the type's)
+    typedef vec<typename T::raw, V> W;
+    const W t = STREAM ? __builtin_nontemporal_load((const W *)p) : *(const W *)p;
 #pragma unroll
     for (int i = 0; i < V; i++) v[i] = (float)t[i];
 }
-template <class T, int V>
+template <class T, int V, bool STREAM = false>
 __device__ __forceinline__ void store(typename T::raw *p, const float (&v)[V])
 {
-    typename T::raw t[V];
+    typedef vec<typename T::raw, V> W;
+    W t;
 #pragma unroll
     for (int i = 0; i < V; i++) t[i] = (typename T::raw)v[i];
-    __builtin_memcpy(p, t, sizeof(t));
+    if (STREAM) __builtin_nontemporal_store(t, (W *)p);
+    else *(W *)p = t;
 }
 
-// the larger magnitude; a NaN wins and stays
-__device__ __forceinline__ double larger(double a, double b) { return a != a ? a : (b != b || b > a) ? b : a; }
+// What the norm sums (fp64 squares: fp32 ones overflow at 1e19) or takes the largest of: magnitudes as the integers that their
+// bits are -- the order is the same, infinity is above all numbers and NaN above infinity.
+struct Squares {
+    using acc = double;
+    __device__ static double of(double a, float x) { return fma((double)x, (double)x, a); }
+    __device__ static double join(double a, double b) { return a + b; }
+    __device__ static double norm(double a) { return sqrt(a); }
+};
+struct Largest {
+    using acc = unsigned;
+    __device__ static unsigned of(unsigned a, float x) { return max(a, __float_as_uint(x) & 0x7fffffffu); }
+    __device__ static unsigned join(unsigned a, unsigned b) { return max(a, b); }
+    __device__ static double norm(unsigned a) { return (double)__uint_as_float(a); }
+};
 
-template <bool MAX>
-__device__ __forceinline__ double join(double a, double b) { return MAX ? larger(a, b) : a + b; }
-
-template <bool MAX>
-__device__ __forceinline__ double block_join(double v, double *lds)
+template <class K>
+__device__ __forceinline__ typename K::acc block_join(typename K::acc v, typename K::acc *lds)
 {
 #pragma unroll
-    for (int o = 32; o; o >>= 1) v = join<MAX>(v, __shfl_xor(v, o));
+    for (int o = 32; o; o >>= 1) v = K::join(v, __shfl_xor(v, o));
     if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
     __syncthreads();
     v = lds[0];
-    for (int i = 1; i < (int)blockDim.x / 64; i++) v = join<MAX>(v, lds[i]);
+    for (int i = 1; i < (int)blockDim.x / 64; i++) v = K::join(v, lds[i]);
     return v;
 }
 
-template <class T, bool MAX>
-__global__ __launch_bounds__(kThreads) void norm_kernel(const Table<1> t, double *part)
+template <class T, class K>
+__global__ __launch_bounds__(kThreads) void norm_kernel(const Table<1> t, typename K::acc *part)
 {
     constexpr int V = 16 / sizeof(typename T::raw);
-    __shared__ double lds[kThreads / 64];
+    __shared__ typename K::acc lds[kThreads / 64];
     const Share s = share(t, blockIdx.x);
     const typename T::raw *g = (const typename T::raw *)t.p[0][s.tensor];
-    double acc[V];
+    typename K::acc acc[V];
 #pragma unroll
     for (int i = 0; i < V; i++) acc[i] = 0;
     int64_t e = s.lo + threadIdx.x * V;
@@ -97,29 +110,27 @@ __global__ __launch_bounds__(kThreads) void norm_kernel(const Table<1> t, double
         float a[V];
         load<T, V>(g + e, a);
 #pragma unroll
-        for (int i = 0; i < V; i++) acc[i] = MAX ? larger(acc[i], fabs((double)a[i])) : fma((double)a[i], (double)a[i], acc[i]);
+        for (int i = 0; i < V; i++) acc[i] = K::of(acc[i], a[i]);
     }
 #pragma unroll
     for (int i = 0; i < V; i++)
-        if (e + i < s.hi) {
-            const double a = (double)(float)g[e + i];
-            acc[i] = MAX ? larger(acc[i], fabs(a)) : fma(a, a, acc[i]);
-        }
+        if (e + i < s.hi) acc[i] = K::of(acc[i], (float)g[e + i]);
 #pragma unroll
-    for (int i = 1; i < V; i++) acc[0] = join<MAX>(acc[0], acc[i]);
-    const double v = block_join<MAX>(acc[0], lds);
+    for (int i = 1; i < V; i++) acc[0] = K::join(acc[0], acc[i]);
+    const typename K::acc v = block_join<K>(acc[0], lds);
     if (threadIdx.x == 0) part[blockIdx.x] = v;
 }
 
-template <bool MAX>
-__global__ __launch_bounds__(1024) void norm_end_kernel(const double *part, int n, float max_norm, float *out)
+template <class K>
+__global__ __launch_bounds__(1024) void norm_end_kernel(const typename K::acc *part, int n, float max_norm, float *out)
 {
-    __shared__ double lds[16];
-    double v = 0;
-    for (int i = threadIdx.x; i < n; i += 1024) v = join<MAX>(v, part[i]);
-    v = block_join<MAX>(v, lds);
+    __shared__ typename K::acc lds[16];
+    typename K::acc v = 0;
+#pragma unroll 8
+    for (int i = threadIdx.x; i < n; i += 1024) v = K::join(v, part[i]);
+    v = block_join<K>(v, lds);
     if (threadIdx.x == 0) {
-        const float norm = (float)(MAX ? v : sqrt(v)), f = max_norm / (norm + 1e-6f);
+        const float norm = (float)K::norm(v), f = max_norm / (norm + 1e-6f);
         out[0] = norm;
         out[1] = max_norm == INFINITY ? 1.f : f > 1.f ? 1.f : f;           // (a NaN stays one)
     }
@@ -160,6 +171,8 @@ __device__ __forceinline__ void adam_value(const Adam &k, float f, float &p, flo
 template <class T>
 __global__ __launch_bounds__(kThreads) void adam_kernel(const Table<4> t, const float *factor, Adam k)
 {
+    // the states are streamed past the cache, where they would push out the weights and gradients (which the next forward and
+    // the norm before read): critic's 317 MB 74.9 -> 63 us; streaming weights and gradients as well: 66-70 us
     constexpr int V = 4;
     const float f = factor ? *factor : 1.f;
     const Share s = share(t, blockIdx.x);
@@ -172,13 +185,13 @@ __global__ __launch_bounds__(kThreads) void adam_kernel(const Table<4> t, const 
         float a[V], b[V], c[V], d[V];
         load<T, V>(p + e, a);
         load<T, V>(g + e, b);
-        load<F32, V>(m + e, c);
-        load<F32, V>(v + e, d);
+        load<F32, V, true>(m + e, c);
+        load<F32, V, true>(v + e, d);
 #pragma unroll
         for (int i = 0; i < V; i++) adam_value(k, f, a[i], b[i], c[i], d[i]);
         store<T, V>(p + e, a);
-        store<F32, V>(m + e, c);
-        store<F32, V>(v + e, d);
+        store<F32, V, true>(m + e, c);
+        store<F32, V, true>(v + e, d);
     }
 #pragma unroll
     for (int i = 0; i < V; i++)
@@ -192,21 +205,17 @@ __global__ __launch_bounds__(kThreads) void adam_kernel(const Table<4> t, const 
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------
-// values per workgroup: enough workgroups to fill the chip eight times over, 4 to 64 accesses of a thread each
-int64_t chunk_of(const int64_t *numels, int n)
+// A launch's values per workgroup: some `workgroups` of them for what its table holds, 4 accesses of a thread at least, 128 at
+// most.  The norm takes 2048, the number that the chip holds at once (1024 / 1536 / 2048 / 3072 / 4096: 45.3 / 42.0 / 42.8 / 47.7 /
+// 44.1 us for the refiner's 214 MB, a last round half empty costing most); the Adam step, whose workgroups move seven streams, four
+// times that (2048 / 4096 / 6144 / 8192: 633 / 619 / 617 / 603 us for 93 million weights).  By the list's total instead, the shorter
+// tables of a long list did not fill the chip (98 us against 85 for the joint model's norm).
+constexpr int kNormWorkgroups = 2048, kAdamWorkgroups = 8192;
+constexpr int64_t kLeast = kThreads * 4 * 4;
+inline int64_t chunk_of(int64_t total, int workgroups)
 {
-    int64_t total = 0;
-    for (int i = 0; i < n; i++) total += numels[i];
-    const int64_t least = kThreads * 4 * 4;
-    int64_t c = (total / 2048 + least - 1) / least * least;
-    return c < least ? least : c > 16 * least ? 16 * least : c;
-}
-
-int64_t blocks_of(const int64_t *numels, int n, int64_t chunk)
-{
-    int64_t b = 0;
-    for (int i = 0; i < n; i++) b += (numels[i] + chunk - 1) / chunk;
-    return b;
+    const int64_t c = (total / workgroups + kLeast - 1) / kLeast * kLeast;
+    return c < kLeast ? kLeast : c > 32 * kLeast ? 32 * kLeast : c;
 }
 
 int check_list(const char *op, const int64_t *numels, const int32_t *dtypes, int n)
@@ -218,7 +227,7 @@ int check_list(const char *op, const int64_t *numels, const int32_t *dtypes, int
         total += numels[i];
         GENRE_REQUIRE(dtypes[i] == GENRE_F32 || dtypes[i] == GENRE_BF16 || dtypes[i] == GENRE_F16, "%s: tensor %d is not fp32, bf16 or fp16", op, i);
     }
-    GENRE_REQUIRE(total / (16 * kThreads * 16) < (1 << 30), "%s: too many values", op);
+    GENRE_REQUIRE(total / (16 * kThreads * 128) < (1 << 30), "%s: too many values", op);
     return 1;
 }
 template <class PTR>
@@ -229,45 +238,78 @@ int check_ptrs(const char *op, const char *what, PTR const *p, const int64_t *nu
     return 1;
 }
 
-// the list cut into tables of one type each; run(table, type, workgroups, workgroups before) launches one
+// the list cut into tables of one type each; run(table, type, workgroups, workgroups before) launches one.  last_first: from the
+// list's end, for a pass behind one that read it from the front -- what that read last is still in the cache (256 MB)
 template <int P, class RUN>
-int each_table(void *const *const (&ptrs)[P], const int64_t *numels, const int32_t *dtypes, int n, const RUN &run)
+int each_table(void *const *const (&ptrs)[P], const int64_t *numels, const int32_t *dtypes, int n, bool last_first, const RUN &run)
 {
     static_assert(sizeof(Table<P>) <= kArgBytes + 64, "a launch's arguments");
     Table<P> t;
-    t.chunk = chunk_of(numels, n);
     int64_t before = 0;
-    for (int type : {GENRE_F32, GENRE_BF16, GENRE_F16}) {
+    for (int j = 0; j < 3; j++) {
+        const int types[3] = {GENRE_F32, GENRE_BF16, GENRE_F16}, type = types[last_first ? 2 - j : j];
+        int64_t total = 0;
         t.n = 0;
-        int64_t blocks = 0;
-        const auto flush = [&]() {
-            if (!t.n) return 1;
-            const int ok = run(t, type, (int)blocks, before);
-            before += blocks;
-            t.n = 0;
-            blocks = 0;
-            return ok;
-        };
-        for (int i = 0; i < n; i++) {
-            if (dtypes[i] != type || !numels[i]) continue;
-            const int64_t b = (numels[i] + t.chunk - 1) / t.chunk;
-            if (t.n == Table<P>::kMost || blocks + b > INT32_MAX)
-                if (!flush()) return 0;
-            for (int j = 0; j < P; j++) t.p[j][t.n] = ptrs[j][i];
-            t.numel[t.n] = numels[i];
-            t.first[t.n] = (int)blocks;
-            t.n++;
-            blocks += b;
+        for (int k = 0; k <= n; k++) {
+            const int i = last_first ? n - 1 - k : k;
+            const bool end = k == n;
+            if (!end && (dtypes[i] != type || !numels[i])) continue;
+            if (t.n == Table<P>::kMost || (end && t.n)) {
+                int64_t blocks = 0;
+                t.chunk = chunk_of(total, P == 1 ? kNormWorkgroups : kAdamWorkgroups);
+                for (int m = 0; m < t.n; m++) {
+                    t.first[m] = (int)blocks;
+                    blocks += (t.numel[m] + t.chunk - 1) / t.chunk;
+                }
+                GENRE_REQUIRE(blocks <= INT32_MAX, "too many values for a launch");
+                if (!run(t, type, (int)blocks, before)) return 0;
+                before += blocks;
+                total = 0;
+                t.n = 0;
+            }
+            if (end) break;
+            for (int m = 0; m < P; m++) t.p[m][t.n] = ptrs[m][i];
+            t.numel[t.n++] = numels[i];
+            total += numels[i];
         }
-        if (!flush()) return 0;
     }
     return 1;
+}
+
+// no fewer than the workgroups of all tables together: each tensor rounds up by less than one, a table's chunk divides its
+// values into kNormWorkgroups or is kLeast or 32 kLeast
+inline int64_t most_blocks(const int64_t *numels, int n)
+{
+    int64_t total = 0;
+    for (int i = 0; i < n; i++) total += numels[i];
+    const int64_t tables = n / Table<1>::kMost + 3, filled = tables * kNormWorkgroups + total / (32 * kLeast), small = total / kLeast;
+    return n + (small < filled ? small : filled);
 }
 
 int check_f32(const char *op, const char *what, const genre_tensor *t, int64_t least)
 {
     GENRE_REQUIRE(t && t->data && t->dtype == GENRE_F32 && is_contiguous(t) && numel(t) >= least,
                   "%s: %s must be a contiguous fp32 tensor of at least %lld values", op, what, (long long)least);
+    return 1;
+}
+
+template <class K>
+int norm_of(const void *const *ptrs, const int64_t *numels, const int32_t *dtypes, int n, float max_norm, float *out, void *ws, hipStream_t st)
+{
+    int64_t blocks = 0;
+    typename K::acc *part = (typename K::acc *)ws;
+    void *const *const lists[1] = {(void *const *)ptrs};
+    const int ok = each_table<1>(lists, numels, dtypes, n, false, [&](const Table<1> &t, int type, int b, int64_t before) {
+        if (type == GENRE_F32) norm_kernel<F32, K><<<b, kThreads, 0, st>>>(t, part + before);
+        else if (type == GENRE_BF16) norm_kernel<BF16, K><<<b, kThreads, 0, st>>>(t, part + before);
+        else norm_kernel<F16, K><<<b, kThreads, 0, st>>>(t, part + before);
+        GENRE_LAUNCH_CHECK("grad norm");
+        blocks = before + b;
+        return 1;
+    });
+    if (!ok) return 0;
+    norm_end_kernel<K><<<1, 1024, 0, st>>>(part, (int)blocks, max_norm, out);
+    GENRE_LAUNCH_CHECK("grad norm end");
     return 1;
 }
 
@@ -279,9 +321,12 @@ using namespace genre;
 extern "C" int64_t genre_grad_workspace(const int64_t *numels, int n)
 {
     if (n < 0 || (n && !numels)) { fail("grad_workspace: the list of sizes is missing"); return -1; }
-    for (int i = 0; i < n; i++)
-        if (numels[i] < 0) { fail("grad_workspace: size %d is negative", i); return -1; }
-    return blocks_of(numels, n, chunk_of(numels, n));
+    int64_t total = 0;
+    for (int i = 0; i < n; i++) {
+        if (numels[i] < 0 || numels[i] >= ((int64_t)1 << 46) - total) { fail("grad_workspace: tensor %d has %lld values", i, (long long)numels[i]); return -1; }
+        total += numels[i];
+    }
+    return most_blocks(numels, n);
 }
 
 extern "C" int genre_grad_norm(const void *const *ptrs, const int64_t *numels, const int32_t *dtypes, int n, int norm_type, float max_norm,
@@ -291,26 +336,13 @@ extern "C" int genre_grad_norm(const void *const *ptrs, const int64_t *numels, c
     if (!check_list(op, numels, dtypes, n) || !check_ptrs(op, "pointer", ptrs, numels, n) || !check_f32(op, "out", out, 2)) return 0;
     GENRE_REQUIRE(norm_type == 2 || norm_type == 0, "%s: norm_type is 2 or 0 (largest magnitude)", op);
     GENRE_REQUIRE(max_norm >= 0, "%s: max_norm must not be negative", op);
-    const int64_t blocks = blocks_of(numels, n, chunk_of(numels, n));
+    const int64_t blocks = most_blocks(numels, n);
     GENRE_REQUIRE(blocks == 0 || (ws && ws->data && ws->dtype == GENRE_F64 && is_contiguous(ws) && numel(ws) >= blocks),
                   "%s: ws must be a contiguous fp64 tensor of at least %lld values", op, (long long)blocks);
     hipStream_t st = (hipStream_t)stream;
-    double *part = blocks ? (double *)ws->data : nullptr;
-    const bool max = norm_type == 0;
-    void *const *const lists[1] = {(void *const *)ptrs};
-    const int ok = each_table<1>(lists, numels, dtypes, n, [&](const Table<1> &t, int type, int b, int64_t before) {
-        double *to = part + before;
-        if (type == GENRE_F32) max ? norm_kernel<F32, true><<<b, kThreads, 0, st>>>(t, to) : norm_kernel<F32, false><<<b, kThreads, 0, st>>>(t, to);
-        else if (type == GENRE_BF16) max ? norm_kernel<BF16, true><<<b, kThreads, 0, st>>>(t, to) : norm_kernel<BF16, false><<<b, kThreads, 0, st>>>(t, to);
-        else max ? norm_kernel<F16, true><<<b, kThreads, 0, st>>>(t, to) : norm_kernel<F16, false><<<b, kThreads, 0, st>>>(t, to);
-        GENRE_LAUNCH_CHECK("grad norm");
-        return 1;
-    });
-    if (!ok) return 0;
-    if (max) norm_end_kernel<true><<<1, 1024, 0, st>>>(part, (int)blocks, max_norm, (float *)out->data);
-    else norm_end_kernel<false><<<1, 1024, 0, st>>>(part, (int)blocks, max_norm, (float *)out->data);
-    GENRE_LAUNCH_CHECK("grad norm end");
-    return 1;
+    void *part = blocks ? ws->data : nullptr;
+    return norm_type == 2 ? norm_of<Squares>(ptrs, numels, dtypes, n, max_norm, (float *)out->data, part, st)
+                          : norm_of<Largest>(ptrs, numels, dtypes, n, max_norm, (float *)out->data, part, st);
 }
 
 extern "C" int genre_grad_scale(void *const *ptrs, const int64_t *numels, const int32_t *dtypes, int n, const genre_tensor *factor, void *stream)
@@ -320,7 +352,7 @@ extern "C" int genre_grad_scale(void *const *ptrs, const int64_t *numels, const 
     hipStream_t st = (hipStream_t)stream;
     const float *f = (const float *)factor->data;
     void *const *const lists[1] = {ptrs};
-    return each_table<1>(lists, numels, dtypes, n, [&](const Table<1> &t, int type, int b, int64_t) {
+    return each_table<1>(lists, numels, dtypes, n, true, [&](const Table<1> &t, int type, int b, int64_t) {
         if (type == GENRE_F32) scale_kernel<F32><<<b, kThreads, 0, st>>>(t, f);
         else if (type == GENRE_BF16) scale_kernel<BF16><<<b, kThreads, 0, st>>>(t, f);
         else scale_kernel<F16><<<b, kThreads, 0, st>>>(t, f);
@@ -353,7 +385,7 @@ extern "C" int genre_adam_step(void *const *p, const void *const *g, void *const
     hipStream_t st = (hipStream_t)stream;
     const float *f = factor ? (const float *)factor->data : nullptr;
     void *const *const lists[4] = {p, (void *const *)g, m, v};
-    return each_table<4>(lists, numels, dtypes, n, [&](const Table<4> &t, int type, int b, int64_t) {
+    return each_table<4>(lists, numels, dtypes, n, true, [&](const Table<4> &t, int type, int b, int64_t) {
         if (type == GENRE_F32) adam_kernel<F32><<<b, kThreads, 0, st>>>(t, f, k);
         else if (type == GENRE_BF16) adam_kernel<BF16><<<b, kThreads, 0, st>>>(t, f, k);
         else adam_kernel<F16><<<b, kThreads, 0, st>>>(t, f, k);
