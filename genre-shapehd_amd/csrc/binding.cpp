@@ -160,12 +160,21 @@ struct Param {
 
 struct Forward { Tensor x, y, stats; };
 
-Tensor scratch(const genre_tensor &x, int64_t groups, int backward, const Tensor &like)
-{
-    const int64_t need = lib.gn_workspace(&x, (int)groups, backward);
-    TORCH_CHECK(need >= 0, lib.last_error());
-    return at::empty({need}, like.options().dtype(at::kDouble));
-}
+// the call's scratch memory, if it needs any
+struct Scratch {
+    Tensor keep;
+    genre_tensor d;
+    const genre_tensor *arg = nullptr;
+    Scratch(const genre_tensor &x, int64_t groups, int backward, const Tensor &like)
+    {
+        const int64_t need = lib.gn_workspace(&x, (int)groups, backward);
+        TORCH_CHECK(need >= 0, lib.last_error());
+        if (!need) return;
+        keep = at::empty({need}, like.options().dtype(at::kDouble));
+        d = flat(keep, GENRE_F64);
+        arg = &d;
+    }
+};
 
 Forward gn_forward(const Tensor &given, const Tensor &weight, const Tensor &bias, int64_t groups, double eps, int64_t act, double slope)
 {
@@ -183,10 +192,9 @@ Forward gn_forward(const Tensor &given, const Tensor &weight, const Tensor &bias
     }
     f.y = like(f.x, in, out);
     const genre_tensor x = map(f.x, in), y = map(f.y, out), stats = flat(f.stats, GENRE_F64);
-    const Tensor ws = scratch(x, groups, 0, given);
-    const genre_tensor w = flat(ws, GENRE_F64);
+    const Scratch ws(x, groups, 0, given);
     const Param p(weight), b(bias);
-    GENRE_CALL("group_norm_act", lib.gn_forward(&x, &y, p.arg, b.arg, &stats, &w, (int)groups, eps, (int)act, (float)slope, stream_of(given)));
+    GENRE_CALL("group_norm_act", lib.gn_forward(&x, &y, p.arg, b.arg, &stats, ws.arg, (int)groups, eps, (int)act, (float)slope, stream_of(given)));
     return f;
 }
 
@@ -231,11 +239,10 @@ public:
             }
             if (ctx->needs_input_grad(0)) dx = like(x, in, out);
             const genre_tensor mx = map(x, in), md = map(dy, grad), st = flat(stats, GENRE_F64), mo = dx.defined() ? map(dx, out) : genre_tensor{};
-            const Tensor ws = scratch(mx, groups, 1, x);
-            const genre_tensor w = flat(ws, GENRE_F64);
+            const Scratch ws(mx, groups, 1, x);
             const Param p(weight), b(bias), gw(dw), gb(db);
             GENRE_CALL("group_norm_act backward",
-                       lib.gn_backward(&mx, &md, p.arg, b.arg, &st, dx.defined() ? &mo : nullptr, gw.arg, gb.arg, &w, (int)groups,
+                       lib.gn_backward(&mx, &md, p.arg, b.arg, &st, dx.defined() ? &mo : nullptr, gw.arg, gb.arg, ws.arg, (int)groups,
                                        (int)ctx->saved_data["act"].toInt(), (float)ctx->saved_data["slope"].toDouble(), stream_of(x)));
         }
         variable_list out = {dx, dw, db, Tensor(), Tensor(), Tensor(), Tensor()};

@@ -10,84 +10,12 @@
 // x less its group's first value, so that sum x^2 / M - mean^2 cancels nothing where the mean is many deviations from zero; z's
 // sign -- which side of its jump a ReLU's derivative takes -- is that of the exact z.  y and dx are rounded once, to their type.  No atomics: partial sums lie in the workspace and are added
 // in a fixed order, so a call's result depends on nothing but its inputs.
-#include "common.hpp"
+#include "group_norm.hpp"
 
 namespace genre {
 namespace {
 
-enum { kActNone = 0, kActRelu = 1, kActLeaky = 2, kActSilu = 3 };
-
-// ---- element types ----------------------------------------------------------------------------------------------
-struct F32 { using raw = float; };
-struct F16 { using raw = _Float16; };
-struct BF16 { using raw = __bf16; };
-
-// V values of type T; the pointer needs no more than T's own alignment (gfx950 loads and stores 16 bytes at any address)
-template <class T, int V>
-__device__ __forceinline__ void load(const typename T::raw *p, float (&v)[V])
-{
-    typename T::raw t[V];
-    __builtin_memcpy(t, p, sizeof(t));
-#pragma unroll
-    for (int i = 0; i < V; i++) v[i] = (float)t[i];
-}
-template <class T, int V>
-__device__ __forceinline__ void store(typename T::raw *p, const float (&v)[V])
-{
-    typename T::raw t[V];
-#pragma unroll
-    for (int i = 0; i < V; i++) t[i] = (typename T::raw)v[i];              // round to nearest even
-    __builtin_memcpy(p, t, sizeof(t));
-}
-
-__device__ __forceinline__ float load_param(const void *p, int dtype, int c, float missing)
-{
-    if (!p) return missing;
-    if (dtype == GENRE_F32) return ((const float *)p)[c];
-    return dtype == GENRE_BF16 ? (float)((const __bf16 *)p)[c] : (float)((const _Float16 *)p)[c];
-}
-__device__ __forceinline__ void store_param(void *p, int dtype, int c, double v)
-{
-    if (dtype == GENRE_F32) ((float *)p)[c] = (float)v;
-    else if (dtype == GENRE_BF16) ((__bf16 *)p)[c] = (__bf16)(float)v;
-    else ((_Float16 *)p)[c] = (_Float16)(float)v;
-}
-
-// ---- activation -------------------------------------------------------------------------------------------------
-// exp and the reciprocal are the hardware's: a few 2^-24 relative around zero, |z| 2^-24 far below it, where the sigmoid is
-// e^-|z| and adds nothing to an output's error
-__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
-
-template <int ACT>
-__device__ __forceinline__ float act_value(double z, float slope)
-{
-    const float f = (float)z;
-    if (ACT == kActRelu) return f > 0.f || f != f ? f : 0.f;
-    if (ACT == kActLeaky) return f > 0.f ? f : f * slope;
-    if (ACT == kActSilu) return f * sigmoid(f);
-    return f;
-}
-template <int ACT>
-__device__ __forceinline__ float act_slope(double z, float slope)
-{
-    if (ACT == kActRelu) return z > 0 ? 1.f : 0.f;
-    if (ACT == kActLeaky) return z > 0 ? 1.f : slope;
-    if (ACT == kActSilu) {
-        const float f = (float)z, s = sigmoid(f);
-        return s * fmaf(f, 1.f - s, 1.f);
-    }
-    return 1.f;
-}
-
-// ---- what the kernels know of a call ----------------------------------------------------------------------------
-struct Map { void *p; int64_t sn, sc, ss; };                               // element strides of image, channel, position
-
-struct Shape {
-    int N, C, G, cg, act;
-    int64_t S;
-    float slope;
-    double m, eps;                                                         // M
-};
+using namespace gn;
 
 // How a channels-last image is cut.  A thread keeps ONE column of V consecutive values and walks down the rows, so that its
 // channels' sums and coefficients stay in registers.  `rows` consecutive rows form a period of `cols` columns: one row where V
@@ -104,31 +32,6 @@ __device__ __forceinline__ Where where(int mids, int chunks)
 {
     const unsigned b = blockIdx.x, m = b / (unsigned)chunks;
     return {(int)(m / (unsigned)mids), (int)(m % (unsigned)mids), (int)(b % (unsigned)chunks)};
-}
-
-__device__ __forceinline__ double wave_sum(double v)
-{
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
-// sum over the workgroup, in every thread; `lds` has 16 doubles; ends with a barrier before lds can be used again
-__device__ __forceinline__ double block_sum(double v, double *lds)
-{
-    v = wave_sum(v);
-    const int waves = (blockDim.x + 63) / 64;
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
-    __syncthreads();
-    double s = 0;
-    for (int i = 0; i < waves; i++) s += lds[i];
-    return s;
-}
-
-template <class T>
-__device__ __forceinline__ double first_value(const Map &x, const Shape &sh, int n, int g)
-{
-    return (double)(float)((const typename T::raw *)x.p)[n * x.sn + (int64_t)g * sh.cg * x.sc];
 }
 
 // per-channel coefficients: z = a (x - mean) + b.  (x - mean first: a value on the mean has z = b exactly, whatever r)
@@ -420,20 +323,6 @@ __global__ __launch_bounds__(256) void group_sums_kernel(Shape sh, int chunks, c
     }
 }
 
-__global__ __launch_bounds__(256) void param_grads_kernel(Shape sh, const double2 *chan, void *dw, int wt, void *db, int bt)
-{
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= sh.C) return;
-    double a = 0, b = 0;
-    for (int n = 0; n < sh.N; n++) {
-        const double2 v = chan[(int64_t)n * sh.C + c];
-        a += v.x;
-        b += v.y;
-    }
-    if (db) store_param(db, bt, c, a);
-    if (dw) store_param(dw, wt, c, b);
-}
-
 // ---- host -------------------------------------------------------------------------------------------------------
 inline bool is_map_type(int32_t t) { return t == GENRE_F32 || t == GENRE_BF16 || t == GENRE_F16; }
 
@@ -458,8 +347,6 @@ inline bool channels_last(const genre_tensor *t) { return t->size[1] == 1 ? t->s
 inline bool channels_first(const genre_tensor *t) { return t->size[2] == 1 || t->stride[2] == 1; }
 inline bool gapless(const genre_tensor *t) { return t->size[2] == 1 || t->stride[2] == t->size[1]; }
 inline Map map_of(const genre_tensor *t) { return {t->data, t->stride[0], t->stride[1], t->size[2] == 1 ? t->size[1] : t->stride[2]}; }
-
-inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 constexpr int kWorkgroups = 2048;                                          // eight of 256 threads for each CU
 
@@ -551,12 +438,11 @@ int64_t workspace_of(const Call &c, bool backward)
 
 int check_f64(const char *op, const char *what, const genre_tensor *t, int64_t least)
 {
-    GENRE_REQUIRE(t && (t->data || least == 0) && t->dtype == GENRE_F64 && is_contiguous(t) && numel(t) >= least,
+    if (least == 0) return 1;
+    GENRE_REQUIRE(t && t->data && t->dtype == GENRE_F64 && is_contiguous(t) && numel(t) >= least,
                   "%s: %s must be a contiguous fp64 tensor of at least %lld values", op, what, (long long)least);
     return 1;
 }
-
-struct Params { const void *w, *b; int wt, bt; };
 
 template <class T, int V, class OP>
 void sums(const Call &c, const Map &x, const Map &dy, const Params &p, const double *stats, double2 *part, hipStream_t st)
@@ -592,8 +478,6 @@ int forward(const Call &c, const Map &x, const Map &y, const Params &p, double *
     GENRE_LAUNCH_CHECK("group norm values");
     return 1;
 }
-
-struct Grads { Map dx; void *dw, *db; int dwt, dbt; };
 
 template <class T, int V, int ACT>
 int backward_as(const Call &c, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
@@ -639,7 +523,8 @@ extern "C" int64_t genre_group_norm_workspace(const genre_tensor *x, int groups,
     Call c{};
     if (!x) { fail("%s: x is NULL", op); return -1; }
     if (!check_map(op, "x", x, x) || !plan(op, x, nullptr, 0, groups, c)) return -1;
-    if (numel(x) == 0) return backward ? 2 * (int64_t)c.sh.N * c.sh.C : 0;
+    if (numel(x) == 0) return 0;
+    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, backward != 0)) return backward ? small_workspace(c.sh) : 0;
     int64_t need = workspace_of(c, backward != 0);
     if (c.last) {                                                          // a gap in another map's rows narrows the columns: room for both
         Call d = c;
@@ -666,14 +551,16 @@ extern "C" int genre_group_norm_forward(const genre_tensor *x, const genre_tenso
     if (!plan(op, x, others, 1, groups, c)) return 0;
     if (!check_f64(op, "stats", stats, 2 * (int64_t)c.sh.N * groups)) return 0;
     if (numel(x) == 0) return 1;
-    if (!check_f64(op, "ws", ws, workspace_of(c, false))) return 0;
     c.sh.act = act;
     c.sh.slope = slope;
     c.sh.eps = eps;
     const Params p = {weight ? weight->data : nullptr, bias ? bias->data : nullptr, weight ? weight->dtype : 0, bias ? bias->dtype : 0};
     const Map mx = map_of(x), my = map_of(y);
-    double *s = (double *)stats->data, *b = (double *)ws->data;
+    double *s = (double *)stats->data;
     hipStream_t st = (hipStream_t)stream;
+    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, false)) return small_forward(c.last, x->dtype, c.sh, mx, my, p, s, st);
+    if (!check_f64(op, "ws", ws, workspace_of(c, false))) return 0;
+    double *b = (double *)ws->data;
     if (x->dtype == GENRE_F32)
         return c.v == 4 ? forward<F32, 4>(c, mx, my, p, s, b, st) : c.v == 2 ? forward<F32, 2>(c, mx, my, p, s, b, st) : forward<F32, 1>(c, mx, my, p, s, b, st);
     if (x->dtype == GENRE_BF16)
@@ -709,13 +596,15 @@ extern "C" int genre_group_norm_backward(const genre_tensor *x, const genre_tens
         }
         return 1;
     }
-    if (!check_f64(op, "ws", ws, workspace_of(c, true))) return 0;
     c.sh.act = act;
     c.sh.slope = slope;
     const Params p = {weight ? weight->data : nullptr, bias ? bias->data : nullptr, weight ? weight->dtype : 0, bias ? bias->dtype : 0};
     const Map mx = map_of(x), md = map_of(dy);
     const double *s = (const double *)stats->data;
-    double *b = (double *)ws->data;
+    const bool small = small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, true);
+    if (!check_f64(op, "ws", ws, small ? small_workspace(c.sh) : workspace_of(c, true))) return 0;
+    double *b = ws ? (double *)ws->data : nullptr;
+    if (small) return small_backward(c.last, x->dtype, c.sh, mx, md, p, g, s, b, st);
     if (x->dtype == GENRE_F32)
         return c.v == 4 ? backward<F32, 4>(c, mx, md, p, g, s, b, st) : c.v == 2 ? backward<F32, 2>(c, mx, md, p, g, s, b, st) : backward<F32, 1>(c, mx, md, p, g, s, b, st);
     if (x->dtype == GENRE_BF16)

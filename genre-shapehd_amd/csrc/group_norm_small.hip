@@ -1,0 +1,391 @@
+// group_norm_small.hip -- group normalisation where one workgroup holds an image's group in its registers.
+//
+// A map whose groups hold up to some 128 (backward: 64) thousand values takes one launch, reads x (and dy) once, and needs no
+// scratch.  A group is `rows` runs of `cols` accesses of V values: channels last, a run is one position's cg channels and every
+// thread keeps one column; channels first, a run is one channel's positions, shared by a team of 2^k threads.
+#include "group_norm.hpp"
+#include <type_traits>
+
+namespace genre {
+namespace {
+
+using namespace gn;
+
+struct Small {
+    int rows, cols, team, deep, turns, subs;                               // threads of a run, runs at once, accesses of a thread and run, waves of a team
+    int64_t gsx, gsd, gso, psx, psd, pso;                             // a run's stride and a group's in x, dy, out (elements)
+};
+
+// a run-time activation: the launches are short, and a kernel for each would be four times as many
+__device__ __forceinline__ float act_of(int act, double z, float slope)
+{
+    switch (act) {
+    case kActRelu: return act_value<kActRelu>(z, slope);
+    case kActLeaky: return act_value<kActLeaky>(z, slope);
+    case kActSilu: return act_value<kActSilu>(z, slope);
+    default: return (float)z;
+    }
+}
+__device__ __forceinline__ float slope_of(int act, double z, float slope)
+{
+    switch (act) {
+    case kActRelu: return act_slope<kActRelu>(z, slope);
+    case kActLeaky: return act_slope<kActLeaky>(z, slope);
+    case kActSilu: return act_slope<kActSilu>(z, slope);
+    default: return 1.f;
+    }
+}
+
+// Workgroups go round the eight dies; a die gets consecutive groups here, so that those of one image, whose channels share
+// cache lines, meet in one L2.
+__device__ __forceinline__ int by_die(int b, int n)
+{
+    const int die = b & 7, each = n >> 3, more = n & 7;
+    return die * each + min(die, more) + (b >> 3);
+}
+
+// V values as they lie in memory: a thread keeps these, two 16-bit values to a register, and converts them in each pass
+template <class T, int V>
+struct Kept {
+    static constexpr int kWords = (V * sizeof(typename T::raw) + 3) / 4;
+    unsigned word[kWords];
+    __device__ void load(const typename T::raw *p)
+    {
+        if (V * sizeof(*p) == 2) word[0] = *(const unsigned short *)p;
+        else __builtin_memcpy(word, p, V * sizeof(*p));
+    }
+    __device__ float at(int i) const
+    {
+        if (sizeof(typename T::raw) == 4) return __uint_as_float(word[i]);
+        const unsigned short h = (unsigned short)(word[i / 2] >> (i % 2 * 16));
+        return (float)__builtin_bit_cast(half_of, h);
+    }
+    // the conversions of one pass are not kept for the next (fp64: two registers a value)
+    __device__ void fresh()
+    {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) asm volatile("" : "+v"(word[i]));
+    }
+    typedef typename std::conditional<sizeof(typename T::raw) == 2, typename T::raw, _Float16>::type half_of;
+};
+
+// a thread's accesses, one after the other: run, column (in accesses), and whether there is one
+template <bool LAST>
+struct Walk {
+    const Small &m;
+    int row, col, turn;
+    bool idle;
+    __device__ explicit Walk(const Small &m) : m(m), idle(LAST && (int)threadIdx.x >= m.team * m.deep) { restart(); }
+    __device__ void restart()
+    {
+        row = threadIdx.x / m.team;
+        col = threadIdx.x % m.team;
+        asm volatile("" : "+v"(row), "+v"(col));                           // (not the last pass's addresses and masks, kept in registers)
+        turn = 0;
+    }
+    __device__ bool here() const { return LAST ? !idle && row < m.rows : row < m.rows && col < m.cols; }
+    __device__ int channel(int v) const { return LAST ? col * v : row; }   // of the access's first value
+    __device__ bool ends_run() const { return turn + 1 == m.turns; }
+    __device__ void next()
+    {
+        if (LAST) {
+            row += m.deep;
+        } else if (++turn == m.turns) {
+            turn = 0;
+            col = threadIdx.x % m.team;
+            row += m.deep;
+        } else {
+            col += m.team;
+        }
+    }
+};
+
+template <class T, int V, int K, bool LAST>
+__global__ __launch_bounds__(1024) void small_forward_kernel(Map x, Map y, Shape sh, Small m, double *stats, const void *w, const void *b, int wt, int bt)
+{
+    using R = typename T::raw;
+    extern __shared__ double coef[];                                       // a and b of the group's channels
+    __shared__ double lds[32];
+    const int id = by_die(blockIdx.x, gridDim.x), n = id / sh.G, g = id % sh.G;
+    const R *px = (const R *)x.p + n * x.sn + g * m.gsx;
+    R *py = (R *)y.p + n * y.sn + g * m.gso;
+    Kept<T, V> v[K];
+    Walk<LAST> at(m);
+#pragma unroll
+    for (int k = 0; k < K; k++, at.next())
+        if (at.here()) v[k].load(px + at.row * m.psx + at.col * V);
+    const double x0 = (double)(float)px[0];
+    double s = 0, q = 0;
+    at.restart();
+#pragma unroll
+    for (int k = 0; k < K; k++, at.next())
+        if (at.here())
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const double d = (double)v[k].at(i) - x0;
+                s += d;
+                q = fma(d, d, q);
+            }
+    block_sum2(s, q, lds);
+    s /= sh.m;
+    q /= sh.m;
+    const double mean = x0 + s, var = fma(-s, s, q), r = 1. / sqrt((var < 0 ? 0. : var) + sh.eps);
+    if (threadIdx.x == 0) {
+        stats[id] = mean;
+        stats[sh.N * sh.G + id] = r;
+    }
+    for (int c = threadIdx.x; c < sh.cg; c += blockDim.x) {
+        coef[c] = r * load_param(w, wt, g * sh.cg + c, 1.f);
+        coef[sh.cg + c] = load_param(b, bt, g * sh.cg + c, 0.f);
+    }
+    __syncthreads();
+    at.restart();
+#pragma unroll
+    for (int k = 0; k < K; k++, at.next()) {
+        if (at.here()) {
+            const int c = at.channel(V);
+            float f[V];
+            v[k].fresh();
+#pragma unroll
+            for (int i = 0; i < V; i++) f[i] = act_of(sh.act, fma((double)v[k].at(i) - mean, coef[c + (LAST ? i : 0)], coef[sh.cg + c + (LAST ? i : 0)]), sh.slope);
+            store<T, V>(py + at.row * m.pso + at.col * V, f);
+        }
+    }
+}
+
+// chan: the sums of dz and dz h by image and channel (more than one image: added up behind this), or dw and db themselves
+template <class T, int V, int K, bool LAST>
+__global__ __launch_bounds__(512) void small_backward_kernel(Map x, Map dy, Map dx, Shape sh, Small m, const double *stats, const void *w, const void *b, int wt,
+                                                             int bt, double2 *chan, void *dw, void *db)
+{
+    using R = typename T::raw;
+    extern __shared__ double coef[];                                       // a, b, w; then the sums' scratch
+    __shared__ double lds[32];
+    const int id = by_die(blockIdx.x, gridDim.x), n = id / sh.G, g = id % sh.G, cg = sh.cg;
+    const R *px = (const R *)x.p + n * x.sn + g * m.gsx, *pd = (const R *)dy.p + n * dy.sn + g * m.gsd;
+    R *po = (R *)dx.p + n * dx.sn + g * m.gso;
+    double2 *scratch = (double2 *)(coef + 3 * cg + (cg & 1));
+    Kept<T, V> v[K], d[K];
+    Walk<LAST> at(m);
+#pragma unroll
+    for (int k = 0; k < K; k++, at.next())
+        if (at.here()) {
+            v[k].load(px + at.row * m.psx + at.col * V);
+            d[k].load(pd + at.row * m.psd + at.col * V);
+        }
+    const double mean = stats[id], r = stats[sh.N * sh.G + id];
+    for (int c = threadIdx.x; c < cg; c += blockDim.x) {
+        const double wc = load_param(w, wt, g * cg + c, 1.f);
+        coef[c] = r * wc;
+        coef[cg + c] = load_param(b, bt, g * cg + c, 0.f);
+        coef[2 * cg + c] = wc;
+    }
+    __syncthreads();
+    // the sums of dz and dz (x - mean) of this thread's channels (last) or of its run (first)
+    double2 acc[LAST ? V : 1];
+#pragma unroll
+    for (int i = 0; i < (LAST ? V : 1); i++) acc[i] = make_double2(0, 0);
+    at.restart();
+#pragma unroll
+    for (int k = 0; k < K; k++, at.next()) {
+        if (at.here()) {
+            const int c = at.channel(V);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int e = LAST ? i : 0;
+                const double h = (double)v[k].at(i) - mean, dz = d[k].at(i) * slope_of(sh.act, fma(h, coef[c + e], coef[cg + c + e]), sh.slope);
+                acc[e].x += dz;
+                acc[e].y = fma(dz, h, acc[e].y);
+            }
+        }
+        if (!LAST && at.ends_run()) {                                       // (uniform) the run's last turn: its team's sum, wave by wave
+            const int lanes = m.team < 64 ? m.team : 64;
+            for (int o = lanes / 2; o; o /= 2) {
+                acc[0].x += __shfl_xor(acc[0].x, o);
+                acc[0].y += __shfl_xor(acc[0].y, o);
+            }
+            if ((int)threadIdx.x % lanes == 0 && at.row < m.rows) scratch[at.row * m.subs + (int)threadIdx.x % m.team / 64] = acc[0];
+            acc[0] = make_double2(0, 0);
+        }
+    }
+    if (LAST) {
+#pragma unroll
+        for (int i = 0; i < V; i++) scratch[i * blockDim.x + threadIdx.x] = acc[i];
+        // a column's threads lie `team` apart: halve their number until one is left
+        int live = m.deep;
+        const int mine = threadIdx.x / m.team;
+        while (live > 1) {
+            const int half = (live + 1) / 2;
+            __syncthreads();
+            if (mine + half < live)
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    double2 &to = scratch[i * blockDim.x + threadIdx.x];
+                    const double2 from = scratch[i * blockDim.x + threadIdx.x + half * m.team];
+                    to.x += from.x;
+                    to.y += from.y;
+                }
+            live = half;
+        }
+    }
+    __syncthreads();
+    double m1 = 0, m2 = 0;
+    for (int c = threadIdx.x; c < cg; c += blockDim.x) {
+        double2 a;
+        if (LAST) {
+            a = scratch[c % V * blockDim.x + c / V];
+        } else {
+            a = scratch[c * m.subs];
+            for (int i = 1; i < m.subs; i++) {
+                a.x += scratch[c * m.subs + i].x;
+                a.y += scratch[c * m.subs + i].y;
+            }
+        }
+        a.y *= r;
+        if (chan) chan[(int64_t)n * sh.C + g * cg + c] = a;
+        if (db) store_param(db, bt, g * cg + c, a.x);
+        if (dw) store_param(dw, wt, g * cg + c, a.y);
+        m1 = fma(coef[2 * cg + c], a.x, m1);
+        m2 = fma(coef[2 * cg + c], a.y, m2);
+    }
+    if (!dx.p) return;                                                     // (uniform)
+    block_sum2(m1, m2, lds);
+    const double k2 = r * (m1 / sh.m), k3 = r * r * (m2 / sh.m);
+    at.restart();
+#pragma unroll
+    for (int k = 0; k < K; k++, at.next()) {
+        if (at.here()) {
+            const int c = at.channel(V);
+            float f[V];
+            v[k].fresh();
+            d[k].fresh();
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const int e = LAST ? i : 0;
+                const double h = (double)v[k].at(i) - mean, dz = d[k].at(i) * slope_of(sh.act, fma(h, coef[c + e], coef[cg + c + e]), sh.slope);
+                f[i] = (float)fma(dz, coef[c + e], -fma(h, k3, k2));
+            }
+            store<T, V>(po + at.row * m.pso + at.col * V, f);
+        }
+    }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------
+// threads of the largest workgroup, 64 values in each: of x (forward), of x and dy (backward)
+constexpr int kMostForward = 1024, kMostBackward = 512;
+
+// the small form of a call, if its groups fit: values per thread 16 or, in the largest workgroups, 64
+struct SmallCall { Small m; int v, values, threads; };
+
+int pow2_from(int64_t n)
+{
+    int p = 1;
+    while (p < n) p *= 2;
+    return p;
+}
+
+bool small_of(bool last, const Shape &sh, int es, int most, const Map &x, const Map &d, const Map &out, SmallCall &c)
+{
+    const int cg = sh.cg;
+    const int64_t S = sh.S;
+    if ((int64_t)cg * S > (int64_t)most * 64 || cg > 1024) return false;
+    const int64_t run = last ? cg : S;
+    c.v = gcd((int)(run & 15), 16 / es);                                   // (run & 15 has run's powers of two up to 8; gcd(0, v) = v)
+    if (c.v == 2) c.v = 1;
+    Small &m = c.m;
+    m.rows = last ? (int)S : cg;
+    m.cols = (int)(run / c.v);
+    m.psx = last ? x.ss : x.sc;
+    m.psd = last ? d.ss : d.sc;
+    m.pso = last ? out.ss : out.sc;
+    m.gsx = cg * x.sc;
+    m.gsd = cg * d.sc;
+    m.gso = cg * out.sc;
+    for (c.values = 16; c.values <= 64; c.values *= 4)
+        for (c.threads = c.values == 16 ? 64 : most; c.threads <= most; c.threads *= 2) {
+            const int k = c.values / c.v;
+            m.turns = m.subs = 1;
+            if (last) {
+                m.team = m.cols;
+                m.deep = c.threads / m.team;
+                if (m.deep && (int64_t)m.deep * k >= m.rows) return true;
+                continue;
+            }
+            for (m.team = pow2_from(m.cols) < c.threads ? pow2_from(m.cols) : c.threads; m.team; m.team /= 2) {
+                m.deep = c.threads / m.team;
+                m.turns = (m.cols + m.team - 1) / m.team;
+                m.subs = m.team > 64 ? m.team / 64 : 1;
+                if (m.turns * ((m.rows + m.deep - 1) / m.deep) <= k) return true;
+            }
+        }
+    return false;
+}
+
+template <class T, int V, bool LAST>
+int forward_as(const Shape &sh, const SmallCall &k, const Map &x, const Map &y, const Params &p, double *stats, hipStream_t st)
+{
+    const size_t lds = 2 * sizeof(double) * sh.cg;
+    const int blocks = sh.N * sh.G;
+    if (k.values == 16) small_forward_kernel<T, V, 16 / V, LAST><<<blocks, k.threads, lds, st>>>(x, y, sh, k.m, stats, p.w, p.b, p.wt, p.bt);
+    else small_forward_kernel<T, V, 64 / V, LAST><<<blocks, k.threads, lds, st>>>(x, y, sh, k.m, stats, p.w, p.b, p.wt, p.bt);
+    GENRE_LAUNCH_CHECK("group norm");
+    return 1;
+}
+
+template <class T, int V, int K, bool LAST>
+int backward_k(const Shape &sh, const SmallCall &k, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
+{
+    static std::atomic<uint64_t> reserved{0};
+    const bool one = sh.N == 1;
+    const size_t lds = sizeof(double) * (3 * sh.cg + (sh.cg & 1)) + sizeof(double2) * (LAST ? V * k.threads : sh.cg * k.m.subs);
+    if (lds > 65536 - 512 && !reserve_lds("group_norm_backward", (const void *)small_backward_kernel<T, V, K, LAST>, 160 * 1024 - 512, reserved)) return 0;
+    double2 *chan = !one && (g.dw || g.db) ? (double2 *)ws : nullptr;
+    small_backward_kernel<T, V, K, LAST><<<sh.N * sh.G, k.threads, lds, st>>>(x, dy, g.dx, sh, k.m, stats, p.w, p.b, p.wt, p.bt, chan, one ? g.dw : nullptr, one ? g.db : nullptr);
+    GENRE_LAUNCH_CHECK("group norm backward");
+    if (chan) {
+        param_grads_kernel<<<ceil_div(sh.C, 256), 256, 0, st>>>(sh, chan, g.dw, g.dwt, g.db, g.dbt);
+        GENRE_LAUNCH_CHECK("group norm parameter gradients");
+    }
+    return 1;
+}
+template <class T, int V, bool LAST>
+int backward_as(const Shape &sh, const SmallCall &k, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
+{
+    return k.values == 16 ? backward_k<T, V, 16 / V, LAST>(sh, k, x, dy, p, g, stats, ws, st) : backward_k<T, V, 64 / V, LAST>(sh, k, x, dy, p, g, stats, ws, st);
+}
+
+
+}  // namespace
+
+namespace gn {
+
+bool small_fits(bool last, const Shape &sh, int es, bool backward)
+{
+    SmallCall k;
+    return small_of(last, sh, es, backward ? kMostBackward : kMostForward, Map{}, Map{}, Map{}, k);
+}
+
+int small_forward(bool last, int dtype, const Shape &sh, const Map &x, const Map &y, const Params &p, double *stats, hipStream_t st)
+{
+    SmallCall k;
+    if (!small_of(last, sh, dtype == GENRE_F32 ? 4 : 2, kMostForward, x, x, y, k)) return fail("group norm: the groups are too large for one workgroup");
+#define GENRE_AS(T, V) (last ? forward_as<T, V, true>(sh, k, x, y, p, stats, st) : forward_as<T, V, false>(sh, k, x, y, p, stats, st))
+    if (dtype == GENRE_F32) return k.v == 4 ? GENRE_AS(F32, 4) : GENRE_AS(F32, 1);
+    if (dtype == GENRE_BF16) return k.v == 8 ? GENRE_AS(BF16, 8) : k.v == 4 ? GENRE_AS(BF16, 4) : GENRE_AS(BF16, 1);
+    return k.v == 8 ? GENRE_AS(F16, 8) : k.v == 4 ? GENRE_AS(F16, 4) : GENRE_AS(F16, 1);
+#undef GENRE_AS
+}
+
+int small_backward(bool last, int dtype, const Shape &sh, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
+{
+    SmallCall k;
+    if (!small_of(last, sh, dtype == GENRE_F32 ? 4 : 2, kMostBackward, x, dy, g.dx, k)) return fail("group norm: the groups are too large for one workgroup");
+#define GENRE_AS(T, V) (last ? backward_as<T, V, true>(sh, k, x, dy, p, g, stats, ws, st) : backward_as<T, V, false>(sh, k, x, dy, p, g, stats, ws, st))
+    if (dtype == GENRE_F32) return k.v == 4 ? GENRE_AS(F32, 4) : GENRE_AS(F32, 1);
+    if (dtype == GENRE_BF16) return k.v == 8 ? GENRE_AS(BF16, 8) : k.v == 4 ? GENRE_AS(BF16, 4) : GENRE_AS(BF16, 1);
+    return k.v == 8 ? GENRE_AS(F16, 8) : k.v == 4 ? GENRE_AS(F16, 4) : GENRE_AS(F16, 1);
+#undef GENRE_AS
+}
+
+}  // namespace gn
+}  // namespace genre

@@ -456,7 +456,7 @@ int genre_render_bm_backward(const genre_tensor *grad_out, const genre_tensor *g
  *   forward:  y = act((x - mean) / sqrt(var + eps) * weight + bias), mean and biased variance of each image and group;
  *             stats fp64 [2,N,groups] receives mean and 1 / sqrt(var + eps)
  *   backward: from x, dy and the forward's stats; dx (NULL: not wanted), dw, db
- * ws: fp64 scratch of at least genre_group_norm_workspace(x, groups, backward) values (-1: refused), undefined before and after;
+ * ws: fp64 scratch of at least genre_group_norm_workspace(x, groups, backward) values (-1: refused; 0: may be NULL), undefined before and after;
  * two calls that may run at once need two.  Sums and statistics are fp64 and added in a fixed order: equal inputs, equal bits.
  * The derivative of (leaky) ReLU at 0 is that of the negative side.  N or S of zero: nothing but dw = db = 0 is written. */
 int64_t genre_group_norm_workspace(const genre_tensor *x, int groups, int backward);

@@ -111,6 +111,9 @@ SHAPES = [
     (1, 1, 1, (4,)), (2, 6, 3, (1, 1, 1)), (2, 8, 2, ()), (1, 5, 5, (33,)), (1, 640, 8, (1, 1, 1)), (2, 12, 12, (3, 3)),
     (3, 20, 4, (5, 7, 3)), (2, 45, 5, (23, 17)), (1, 1, 1, (70, 3)), (1, 1023, 3, (3, 5)), (2, 1030, 2, (9,)), (1, 4104, 8, (2, 3)),
     (1, 16, 1, (1, 2, 3)), (9, 3, 3, (2,)), (2, 80, 8, (16, 15, 14)),
+    # groups of more values than one workgroup holds (65536 forward, 32768 backward), of more channels, and at the border
+    (2, 45, 1, (41, 40)), (1, 511, 1, (13, 11)), (1, 1030, 2, (9, 15)), (1, 1030, 1, (3,)), (1, 4104, 2, (5, 7)), (2, 7, 1, (101, 97)), (1, 3, 1, (40001,)),
+    (1, 64, 2, (32, 32)), (1, 64, 2, (32, 33)), (1, 64, 1, (32, 32)), (1, 64, 1, (32, 33)), (1, 96, 1, (700,)),
 ]
 
 
