@@ -21,38 +21,76 @@ using namespace gn;
 // channels' sums and coefficients stay in registers.  `rows` consecutive rows form a period of `cols` columns: one row where V
 // divides C, else (rows without gaps only) the V / gcd(C, V) rows after which the columns fall on the same channels again.
 struct Cut {
-    int rows, cols, tile, tiles, deep, threads;                            // columns per workgroup, tiles of a period; periods side by side
+    int rows, cols, tile, tiles, deep;                                     // columns per workgroup, tiles of a period; periods side by side
     int64_t periods, per;                                                  // whole and part periods of an image, per workgroup
     int chunks;
 };
+struct Run { int64_t per; int chunks; };                                   // channels first: positions per workgroup
 
 // one workgroup's share of a map: image, chunk and (channels last) tile or (channels first) channel
 struct Where { int n, mid, chunk; };
-__device__ __forceinline__ Where where(int mids, int chunks)
+__device__ __forceinline__ Where where(unsigned b, int mids, int chunks)
 {
-    const unsigned b = blockIdx.x, m = b / (unsigned)chunks;
+    const unsigned m = b / (unsigned)chunks;
     return {(int)(m / (unsigned)mids), (int)(m % (unsigned)mids), (int)(b % (unsigned)chunks)};
 }
 
-// per-channel coefficients: z = a (x - mean) + b.  (x - mean first: a value on the mean has z = b exactly, whatever r)
-struct Norm { double mean, a, b, r; };
-__device__ __forceinline__ Norm norm_of(const double *stats, const Shape &sh, int n, int c, float w, float bias)
+// statistics of an image's group, and for dx the means of w dz and w dz h over it
+struct Stat { double mean, r, m1, m2; };
+
+// The chunks' sums and what becomes of them: statistics (forward, with x0) or m1 and m2 (backward).  `joined`: every workgroup of
+// the second pass adds up its groups' sums itself, some 1000 pairs at most; otherwise a launch between the passes has done so.
+struct Between {
+    bool joined;
+    int chunks;                                                            // of the first pass
+    const double2 *chan, *group;                                           // [image][chunk][channel]; channels last: [image][chunk][group]
+    double *stats;                                                         // [2][image][group]
+    const double *sums;                                                    // [image][group][2], where not joined
+    void *dw, *db;
+    int dwt, dbt;
+    unsigned blocks;                                                       // of the map; those behind them see to dw and db
+};
+
+template <class T>
+__device__ __forceinline__ Stat stat_of(const Map &x, const Shape &sh, int n, int g, double s, double q)
 {
-    const int at = n * sh.G + c / sh.cg;
-    const double r = stats[sh.N * sh.G + at];
-    return {stats[at], r * w, bias, r};
+    const double d = s / sh.m, var = fma(-d, d, q / sh.m);
+    return {first_value<T>(x, sh, n, g) + d, 1. / sqrt((var < 0 ? 0. : var) + sh.eps), 0, 0};      // (equal values: the mean is theirs, exactly; a NaN stays one)
+}
+__device__ __forceinline__ void keep_stat(const Shape &sh, double *stats, int at, const Stat &t)
+{
+    stats[at] = t.mean;
+    stats[sh.N * sh.G + at] = t.r;
+}
+__device__ __forceinline__ Stat saved_stat(const Shape &sh, const Between &k, int at, bool two)
+{
+    return {k.stats[at], k.stats[sh.N * sh.G + at], two && !k.joined ? k.sums[2 * at] : 0, two && !k.joined ? k.sums[2 * at + 1] : 0};
+}
+// the sum of a group's pairs over its channels and all chunks, in every thread
+template <bool TWO>
+__device__ __forceinline__ double2 group_total(const Shape &sh, int chunks, const double2 *chan, int n, int g, const void *w, int wt, double *lds)
+{
+    const double2 *p = chan + (int64_t)n * chunks * sh.C + g * sh.cg;
+    double2 t = make_double2(0, 0);
+    for (unsigned i = threadIdx.x; i < (unsigned)chunks * sh.cg; i += blockDim.x) {
+        const unsigned row = i / (unsigned)sh.cg, c = i % (unsigned)sh.cg;
+        const double2 v = p[(int64_t)row * sh.C + c];
+        const double f = TWO ? load_param(w, wt, g * sh.cg + c, 1.f) : 1.f;
+        t.x = fma(f, v.x, t.x);
+        t.y = fma(f, v.y, t.y);
+    }
+    block_sum2(t.x, t.y, lds);
+    return t;
 }
 
 // ---- what one value contributes (the loops over a map are written once, for each of these) ----------------------
-// forward sums: d, d^2 of d = x - x0, x0 the group's first value
+// Coef: what a channel of an image needs, made once per workgroup.  z = a (x - mean) + b, a = r w: a value on the mean has z = b
+// exactly, whatever r.
 template <class T>
-struct SumsF {
+struct SumsF {                                                             // d and d^2 of d = x - x0, x0 the group's first value
     static constexpr bool kTwo = false;
     struct Coef { double x0; };
-    __device__ static Coef coef(const Map &x, const Shape &sh, const double *, int n, int c, const void *, const void *, int, int)
-    {
-        return {first_value<T>(x, sh, n, c / sh.cg)};
-    }
+    __device__ static Coef coef(double x0, const Stat &, float, float) { return {x0}; }
     __device__ static void add(const Coef &k, float, float x, float, double &s, double &q)
     {
         const double d = (double)x - k.x0;
@@ -60,20 +98,14 @@ struct SumsF {
         q = fma(d, d, q);
     }
 };
-// backward sums: dz, dz (x - mean)
 template <class T, int ACT>
-struct SumsB {
+struct SumsB {                                                             // dz and dz (x - mean)
     static constexpr bool kTwo = true;
     struct Coef { double mean, a, b; };
-    __device__ static Coef coef(const Map &, const Shape &sh, const double *stats, int n, int c, const void *w, const void *b, int wt, int bt)
-    {
-        const Norm k = norm_of(stats, sh, n, c, load_param(w, wt, c, 1.f), load_param(b, bt, c, 0.f));
-        return {k.mean, k.a, k.b};
-    }
+    __device__ static Coef coef(double, const Stat &t, float w, float b) { return {t.mean, t.r * w, b}; }
     __device__ static void add(const Coef &k, float slope, float x, float dy, double &s, double &q)
     {
-        const double d = (double)x - k.mean;
-        const double dz = dy * act_slope<ACT>(fma(d, k.a, k.b), slope);
+        const double d = (double)x - k.mean, dz = dy * act_slope<ACT>(fma(d, k.a, k.b), slope);
         s += dz;
         q = fma(dz, d, q);
     }
@@ -82,26 +114,14 @@ template <class T, int ACT>
 struct ValueF {
     static constexpr bool kTwo = false;
     struct Coef { double mean, a, b; };
-    __device__ static Coef coef(const Shape &sh, const double *stats, const double *, int n, int c, const void *w, const void *b, int wt, int bt)
-    {
-        const Norm k = norm_of(stats, sh, n, c, load_param(w, wt, c, 1.f), load_param(b, bt, c, 0.f));
-        return {k.mean, k.a, k.b};
-    }
-    __device__ static float value(const Coef &k, float slope, float x, float)
-    {
-        return act_value<ACT>(fma((double)x - k.mean, k.a, k.b), slope);
-    }
+    __device__ static Coef coef(const Stat &t, float w, float b) { return {t.mean, t.r * w, b}; }
+    __device__ static float value(const Coef &k, float slope, float x, float) { return act_value<ACT>(fma((double)x - k.mean, k.a, k.b), slope); }
 };
 template <class T, int ACT>
 struct ValueB {
     static constexpr bool kTwo = true;
     struct Coef { double mean, a, b, k2, k3; };                            // dx = a dz - (k3 (x - mean) + k2)
-    __device__ static Coef coef(const Shape &sh, const double *stats, const double *sums, int n, int c, const void *w, const void *b, int wt, int bt)
-    {
-        const Norm k = norm_of(stats, sh, n, c, load_param(w, wt, c, 1.f), load_param(b, bt, c, 0.f));
-        const int at = n * sh.G + c / sh.cg;
-        return {k.mean, k.a, k.b, k.r * sums[2 * at], k.r * k.r * sums[2 * at + 1]};
-    }
+    __device__ static Coef coef(const Stat &t, float w, float b) { return {t.mean, t.r * w, b, t.r * t.m1, t.r * t.r * t.m2}; }
     __device__ static float value(const Coef &k, float slope, float x, float dy)
     {
         const double d = (double)x - k.mean, dz = dy * act_slope<ACT>(fma(d, k.a, k.b), slope);
@@ -109,33 +129,75 @@ struct ValueB {
     }
 };
 
+constexpr int kBatch = 4;                                                  // accesses of a thread in flight at once
+
 // ---- channels last ----------------------------------------------------------------------------------------------
+// the coefficients of a thread's V channels: its column's, made by one thread each where a workgroup has several periods side by
+// side (`lds`: room for a tile's), else by the thread itself
+template <int V, class COEF, class MAKE>
+__device__ __forceinline__ void column_coefs(COEF (&k)[V], COEF *lds, const Shape &sh, const Cut &cut, int tile, int in, const MAKE &make)
+{
+    const int first = cut.rows == 1 ? tile * cut.tile * V : 0, many = cut.rows == 1 ? min(cut.tile * V, sh.C - first) : sh.C;
+    const bool own = cut.deep == 1 && cut.rows == 1;
+    if (!own) {
+        for (int j = threadIdx.x; j < many; j += blockDim.x) lds[j] = make(first + j);
+        __syncthreads();
+    }
+    int c = in * V % (own ? sh.C : many);                                  // (one row a period: below `many` but in idle threads)
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        if (own) k[i] = make(min(first + c, sh.C - 1));
+        else k[i] = lds[c];
+        if (++c == (own ? sh.C : many)) c = 0;
+    }
+}
+// how many bytes of LDS that takes, with `coef` bytes a channel
+inline size_t coef_bytes(const Shape &sh, const Cut &cut, int v, size_t coef)
+{
+    if (cut.deep == 1 && cut.rows == 1) return 0;
+    return coef * (cut.rows == 1 ? (cut.tile * v < sh.C ? cut.tile * v : sh.C) : sh.C);
+}
+
 template <class T, int V, class OP>
-__global__ __launch_bounds__(512) void last_sums_kernel(Map x, Map dy, Shape sh, Cut cut, const double *stats, const void *w, const void *b,
-                                                        int wt, int bt, double2 *part)
+__global__ __launch_bounds__(512) void last_sums_kernel(Map x, Map dy, Shape sh, Cut cut, Between bt, const void *w, const void *b, int wt, int bty,
+                                                        double2 *chan, double2 *group)
 {
     using R = typename T::raw;
     extern __shared__ double lds[];
-    const Where at = where(cut.tiles, cut.chunks);
+    const Where at = where(blockIdx.x, cut.tiles, cut.chunks);
     const int r = threadIdx.x / cut.tile, in = threadIdx.x % cut.tile, col = at.mid * cut.tile + in;
+    typename OP::Coef k[V];
+    column_coefs<V>(k, (typename OP::Coef *)lds, sh, cut, at.mid, in, [&](int c) {
+        const int g = c / sh.cg;
+        return OP::kTwo ? OP::coef(0, saved_stat(sh, bt, at.n * sh.G + g, false), load_param(w, wt, c, 1.f), load_param(b, bty, c, 0.f))
+                        : OP::coef(first_value<T>(x, sh, at.n, g), Stat{}, 0, 0);
+    });
     double s[V], q[V];
 #pragma unroll
     for (int i = 0; i < V; i++) s[i] = q[i] = 0;
     if (r < cut.deep && col < cut.cols) {
-        typename OP::Coef k[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) k[i] = OP::coef(x, sh, stats, at.n, (col * V + i) % sh.C, w, b, wt, bt);
         const int64_t lo = at.chunk * cut.per, hi = min(lo + cut.per, cut.periods), whole = min(hi, sh.S / cut.rows);
-        const R *px = (const R *)x.p + at.n * x.sn + col * V, *pd = (const R *)dy.p + (OP::kTwo ? at.n * dy.sn + col * V : 0);
+        const R *px = (const R *)x.p + at.n * x.sn + col * V, *pd = OP::kTwo ? (const R *)dy.p + at.n * dy.sn + col * V : nullptr;
         const int64_t dx = cut.rows * x.ss, dd = cut.rows * dy.ss;
         int64_t p = lo + r;
-#pragma unroll 4
-        for (; p < whole; p += cut.deep) {
-            float a[V], d[V] = {};
-            load<T, V>(px + p * dx, a);
-            if (OP::kTwo) load<T, V>(pd + p * dd, d);
+        for (; p + (kBatch - 1) * cut.deep < whole; p += kBatch * cut.deep) {
+            Kept<T, V> a[kBatch], d[kBatch];
 #pragma unroll
-            for (int i = 0; i < V; i++) OP::add(k[i], sh.slope, a[i], d[i], s[i], q[i]);
+            for (int u = 0; u < kBatch; u++) {
+                a[u].load(px + (p + u * cut.deep) * dx);
+                if (OP::kTwo) d[u].load(pd + (p + u * cut.deep) * dd);
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; u++)
+#pragma unroll
+                for (int i = 0; i < V; i++) OP::add(k[i], sh.slope, a[u].at(i), OP::kTwo ? d[u].at(i) : 0.f, s[i], q[i]);
+        }
+        for (; p < whole; p += cut.deep) {
+            Kept<T, V> a, d;
+            a.load(px + p * dx);
+            if (OP::kTwo) d.load(pd + p * dd);
+#pragma unroll
+            for (int i = 0; i < V; i++) OP::add(k[i], sh.slope, a.at(i), OP::kTwo ? d.at(i) : 0.f, s[i], q[i]);
         }
         if (p < hi) {                                                      // the part period behind the last whole one
             const int64_t left = (sh.S - p * cut.rows) * sh.C - col * V;
@@ -144,51 +206,122 @@ __global__ __launch_bounds__(512) void last_sums_kernel(Map x, Map dy, Shape sh,
                 if (i < left) OP::add(k[i], sh.slope, (float)px[p * dx + i], OP::kTwo ? (float)pd[p * dd + i] : 0.f, s[i], q[i]);
         }
     }
-    // [sum][i][thread]: a channel's column is a period's value e = channel + m C, in each of `deep` periods
+    __syncthreads();
+    // [i][thread] pairs, halved until one period is left; then a channel is its period's values e = channel + m C
+    double2 *pair = (double2 *)lds;
     const int T0 = blockDim.x;
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        lds[i * T0 + threadIdx.x] = s[i];
-        lds[(V + i) * T0 + threadIdx.x] = q[i];
+    for (int i = 0; i < V; i++) pair[i * T0 + threadIdx.x] = make_double2(s[i], q[i]);
+    for (int live = cut.deep; live > 1;) {
+        const int half = (live + 1) / 2;
+        __syncthreads();
+        if (r + half < live)
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const double2 from = pair[i * T0 + threadIdx.x + half * cut.tile];
+                s[i] += from.x;
+                q[i] += from.y;
+                pair[i * T0 + threadIdx.x] = make_double2(s[i], q[i]);
+            }
+        live = half;
     }
     __syncthreads();
     const int first = cut.rows == 1 ? at.mid * cut.tile * V : 0, many = cut.rows == 1 ? min(cut.tile * V, sh.C - first) : sh.C;
+    const int64_t row = (int64_t)at.n * cut.chunks + at.chunk;
+    double2 *mine = pair + V * T0;                                         // (with `group`: a tile is all channels)
     for (int j = threadIdx.x; j < many; j += T0) {
-        double a = 0, c = 0;
-        for (int m = 0; m < cut.rows; m++) {
-            const int e = j + m * sh.C, o = (e % V) * T0 + e / V;
-            for (int d = 0; d < cut.deep; d++) {
-                a += lds[o + d * cut.tile];
-                c += lds[V * T0 + o + d * cut.tile];
-            }
+        double2 t = make_double2(0, 0);
+        for (int m = 0, e = j; m < cut.rows; m++, e += sh.C) {
+            const double2 v = pair[e % V * T0 + e / V];
+            t.x += v.x;
+            t.y += v.y;
         }
-        part[((int64_t)at.n * cut.chunks + at.chunk) * sh.C + first + j] = make_double2(a, c);
+        if (chan) chan[row * sh.C + first + j] = t;
+        if (group) {
+            const double f = OP::kTwo ? load_param(w, wt, j, 1.f) : 1.f;
+            mine[j] = make_double2(f * t.x, f * t.y);
+        }
+    }
+    if (!group) return;                                                    // (uniform)
+    __syncthreads();
+    for (int g = threadIdx.x; g < sh.G; g += T0) {
+        double2 t = make_double2(0, 0);
+        for (int j = 0; j < sh.cg; j++) {
+            t.x += mine[g * sh.cg + j].x;
+            t.y += mine[g * sh.cg + j].y;
+        }
+        group[row * sh.G + g] = t;
     }
 }
 
+constexpr int kJoinedGroups = 64;
+
 template <class T, int V, class OP>
-__global__ __launch_bounds__(512) void last_value_kernel(Map x, Map dy, Map out, Shape sh, Cut cut, const double *stats, const double *sums,
-                                                         const void *w, const void *b, int wt, int bt)
+__global__ __launch_bounds__(512) void last_value_kernel(Map x, Map dy, Map out, Shape sh, Cut cut, Between bt, const void *w, const void *b, int wt, int bty)
 {
     using R = typename T::raw;
-    const Where at = where(cut.tiles, cut.chunks);
+    extern __shared__ double lds[];
+    __shared__ double2 total[512];
+    __shared__ Stat stat[kJoinedGroups];
+    if (OP::kTwo && blockIdx.x >= bt.blocks) {
+        const int c = (blockIdx.x - bt.blocks) * (blockDim.x / 64) + threadIdx.x / 64;
+        if (c < sh.C) channel_grads(sh, bt.chunks, bt.chan, bt.stats, c, bt.dw, bt.dwt, bt.db, bt.dbt);
+        return;
+    }
+    const Where at = where(bt.blocks - 1 - blockIdx.x, cut.tiles, cut.chunks);           // from the end: what the first pass read last is still in the cache
+    if (bt.joined) {
+        const int each = blockDim.x / sh.G, g = threadIdx.x % sh.G, lane = threadIdx.x / sh.G;
+        double2 t = make_double2(0, 0);
+        if (lane < each)
+            for (int i = lane; i < bt.chunks; i += each) {
+                const double2 v = bt.group[((int64_t)at.n * bt.chunks + i) * sh.G + g];
+                t.x += v.x;
+                t.y += v.y;
+            }
+        total[threadIdx.x] = t;
+        for (int live = each; live > 1;) {
+            const int half = (live + 1) / 2;
+            __syncthreads();
+            if (lane + half < live) {
+                t.x += total[threadIdx.x + half * sh.G].x;
+                t.y += total[threadIdx.x + half * sh.G].y;
+                total[threadIdx.x] = t;
+            }
+            live = half;
+        }
+        if (lane == 0) {
+            const int i = at.n * sh.G + g;
+            if (OP::kTwo) {
+                Stat v = saved_stat(sh, bt, i, true);
+                v.m1 = t.x / sh.m;
+                v.m2 = t.y * v.r / sh.m;
+                stat[g] = v;
+            } else {
+                stat[g] = stat_of<T>(x, sh, at.n, g, t.x, t.y);
+                if (at.chunk == 0) keep_stat(sh, bt.stats, i, stat[g]);
+            }
+        }
+        __syncthreads();
+    }
     const int r = threadIdx.x / cut.tile, in = threadIdx.x % cut.tile, col = at.mid * cut.tile + in;
-    if (r >= cut.deep || col >= cut.cols) return;
     typename OP::Coef k[V];
-#pragma unroll
-    for (int i = 0; i < V; i++) k[i] = OP::coef(sh, stats, sums, at.n, (col * V + i) % sh.C, w, b, wt, bt);
+    column_coefs<V>(k, (typename OP::Coef *)lds, sh, cut, at.mid, in, [&](int c) {
+        const int g = c / sh.cg;
+        return OP::coef(bt.joined ? stat[g] : saved_stat(sh, bt, at.n * sh.G + g, OP::kTwo), load_param(w, wt, c, 1.f), load_param(b, bty, c, 0.f));
+    });
+    if (r >= cut.deep || col >= cut.cols) return;
     const int64_t lo = at.chunk * cut.per, hi = min(lo + cut.per, cut.periods), whole = min(hi, sh.S / cut.rows);
-    const R *px = (const R *)x.p + at.n * x.sn + col * V, *pd = (const R *)dy.p + (OP::kTwo ? at.n * dy.sn + col * V : 0);
+    const R *px = (const R *)x.p + at.n * x.sn + col * V, *pd = OP::kTwo ? (const R *)dy.p + at.n * dy.sn + col * V : nullptr;
     R *po = (R *)out.p + at.n * out.sn + col * V;
     const int64_t dx = cut.rows * x.ss, dd = cut.rows * dy.ss, dout = cut.rows * out.ss;
     int64_t p = lo + r;
-#pragma unroll 4
     for (; p < whole; p += cut.deep) {
-        float a[V], d[V] = {}, v[V];
-        load<T, V>(px + p * dx, a);
-        if (OP::kTwo) load<T, V>(pd + p * dd, d);
+        Kept<T, V> a, d;
+        float v[V];
+        a.load(px + p * dx);
+        if (OP::kTwo) d.load(pd + p * dd);
 #pragma unroll
-        for (int i = 0; i < V; i++) v[i] = OP::value(k[i], sh.slope, a[i], d[i]);
+        for (int i = 0; i < V; i++) v[i] = OP::value(k[i], sh.slope, a.at(i), OP::kTwo ? d.at(i) : 0.f);
         store<T, V>(po + p * dout, v);
     }
     if (p < hi) {
@@ -202,124 +335,110 @@ __global__ __launch_bounds__(512) void last_value_kernel(Map x, Map dy, Map out,
 
 // ---- channels first ---------------------------------------------------------------------------------------------
 template <class T, int V, class OP>
-__global__ __launch_bounds__(256) void first_sums_kernel(Map x, Map dy, Shape sh, int chunks, int64_t per, const double *stats, const void *w,
-                                                         const void *b, int wt, int bt, double2 *part)
+__global__ __launch_bounds__(256) void first_sums_kernel(Map x, Map dy, Shape sh, Run run, Between bt, const void *w, const void *b, int wt, int bty, double2 *chan)
 {
     using R = typename T::raw;
-    __shared__ double lds[16];
-    const Where at = where(sh.C, chunks);
-    const typename OP::Coef k = OP::coef(x, sh, stats, at.n, at.mid, w, b, wt, bt);
-    const R *px = (const R *)x.p + at.n * x.sn + at.mid * x.sc, *pd = (const R *)dy.p + (OP::kTwo ? at.n * dy.sn + at.mid * dy.sc : 0);
-    const int64_t hi = min((at.chunk + 1) * per, sh.S);
-    double s[V], q[V];
+    __shared__ double lds[32];
+    const Where at = where(blockIdx.x, sh.C, run.chunks);
+    const int g = at.mid / sh.cg;
+    const typename OP::Coef k = OP::kTwo ? OP::coef(0, saved_stat(sh, bt, at.n * sh.G + g, false), load_param(w, wt, at.mid, 1.f), load_param(b, bty, at.mid, 0.f))
+                                         : OP::coef(first_value<T>(x, sh, at.n, g), Stat{}, 0, 0);
+    const R *px = (const R *)x.p + at.n * x.sn + at.mid * x.sc, *pd = OP::kTwo ? (const R *)dy.p + at.n * dy.sn + at.mid * dy.sc : nullptr;
+    const int64_t hi = min((at.chunk + 1) * run.per, sh.S);
+    const int step = blockDim.x * V;
+    double s[2] = {0, 0}, q[2] = {0, 0};
+    int64_t e = at.chunk * run.per + threadIdx.x * V;
+    for (; e + (kBatch - 1) * step + V <= hi; e += kBatch * step) {
+        Kept<T, V> a[kBatch], d[kBatch];
 #pragma unroll
-    for (int i = 0; i < V; i++) s[i] = q[i] = 0;
-    int64_t e = at.chunk * per + threadIdx.x * V;
-#pragma unroll 4
-    for (; e + V <= hi; e += blockDim.x * V) {
-        float a[V], d[V] = {};
-        load<T, V>(px + e, a);
-        if (OP::kTwo) load<T, V>(pd + e, d);
+        for (int u = 0; u < kBatch; u++) {
+            a[u].load(px + e + u * step);
+            if (OP::kTwo) d[u].load(pd + e + u * step);
+        }
 #pragma unroll
-        for (int i = 0; i < V; i++) OP::add(k, sh.slope, a[i], d[i], s[i], q[i]);
+        for (int u = 0; u < kBatch; u++)
+#pragma unroll
+            for (int i = 0; i < V; i++) OP::add(k, sh.slope, a[u].at(i), OP::kTwo ? d[u].at(i) : 0.f, s[i & 1], q[i & 1]);
+    }
+    for (; e + V <= hi; e += step) {
+        Kept<T, V> a, d;
+        a.load(px + e);
+        if (OP::kTwo) d.load(pd + e);
+#pragma unroll
+        for (int i = 0; i < V; i++) OP::add(k, sh.slope, a.at(i), OP::kTwo ? d.at(i) : 0.f, s[i & 1], q[i & 1]);
     }
 #pragma unroll
     for (int i = 0; i < V; i++)
-        if (e + i < hi) OP::add(k, sh.slope, (float)px[e + i], OP::kTwo ? (float)pd[e + i] : 0.f, s[i], q[i]);
-#pragma unroll
-    for (int i = 1; i < V; i++) { s[0] += s[i]; q[0] += q[i]; }
-    const double a = block_sum(s[0], lds), c = block_sum(q[0], lds);
-    if (threadIdx.x == 0) part[((int64_t)at.n * chunks + at.chunk) * sh.C + at.mid] = make_double2(a, c);
+        if (e + i < hi) OP::add(k, sh.slope, (float)px[e + i], OP::kTwo ? (float)pd[e + i] : 0.f, s[i & 1], q[i & 1]);
+    s[0] += s[1];
+    q[0] += q[1];
+    block_sum2(s[0], q[0], lds);
+    if (threadIdx.x == 0) chan[((int64_t)at.n * run.chunks + at.chunk) * sh.C + at.mid] = make_double2(s[0], q[0]);
 }
 
 template <class T, int V, class OP>
-__global__ __launch_bounds__(256) void first_value_kernel(Map x, Map dy, Map out, Shape sh, int chunks, int64_t per, const double *stats,
-                                                          const double *sums, const void *w, const void *b, int wt, int bt)
+__global__ __launch_bounds__(256) void first_value_kernel(Map x, Map dy, Map out, Shape sh, Run run, Between bt, const void *w, const void *b, int wt, int bty)
 {
     using R = typename T::raw;
-    const Where at = where(sh.C, chunks);
-    const typename OP::Coef k = OP::coef(sh, stats, sums, at.n, at.mid, w, b, wt, bt);
-    const R *px = (const R *)x.p + at.n * x.sn + at.mid * x.sc, *pd = (const R *)dy.p + (OP::kTwo ? at.n * dy.sn + at.mid * dy.sc : 0);
+    __shared__ double lds[32];
+    if (OP::kTwo && blockIdx.x >= bt.blocks) {
+        const int c = (blockIdx.x - bt.blocks) * (blockDim.x / 64) + threadIdx.x / 64;
+        if (c < sh.C) channel_grads(sh, bt.chunks, bt.chan, bt.stats, c, bt.dw, bt.dwt, bt.db, bt.dbt);
+        return;
+    }
+    const Where at = where(bt.blocks - 1 - blockIdx.x, sh.C, run.chunks);
+    const int g = at.mid / sh.cg, i = at.n * sh.G + g;
+    Stat t;
+    if (bt.joined) {
+        const double2 v = group_total<OP::kTwo>(sh, bt.chunks, bt.chan, at.n, g, w, wt, lds);
+        if (OP::kTwo) {
+            t = saved_stat(sh, bt, i, true);
+            t.m1 = v.x / sh.m;
+            t.m2 = v.y * t.r / sh.m;
+        } else {
+            t = stat_of<T>(x, sh, at.n, g, v.x, v.y);
+            if (at.chunk == 0 && at.mid == g * sh.cg && threadIdx.x == 0) keep_stat(sh, bt.stats, i, t);
+        }
+    } else {
+        t = saved_stat(sh, bt, i, OP::kTwo);
+    }
+    const typename OP::Coef k = OP::coef(t, load_param(w, wt, at.mid, 1.f), load_param(b, bty, at.mid, 0.f));
+    const R *px = (const R *)x.p + at.n * x.sn + at.mid * x.sc, *pd = OP::kTwo ? (const R *)dy.p + at.n * dy.sn + at.mid * dy.sc : nullptr;
     R *po = (R *)out.p + at.n * out.sn + at.mid * out.sc;
-    const int64_t hi = min((at.chunk + 1) * per, sh.S);
-    int64_t e = at.chunk * per + threadIdx.x * V;
-#pragma unroll 4
-    for (; e + V <= hi; e += blockDim.x * V) {
-        float a[V], d[V] = {}, v[V];
-        load<T, V>(px + e, a);
-        if (OP::kTwo) load<T, V>(pd + e, d);
+    const int64_t hi = min((at.chunk + 1) * run.per, sh.S);
+    const int step = blockDim.x * V;
+    int64_t e = at.chunk * run.per + threadIdx.x * V;
+    for (; e + V <= hi; e += step) {
+        Kept<T, V> a, d;
+        float v[V];
+        a.load(px + e);
+        if (OP::kTwo) d.load(pd + e);
 #pragma unroll
-        for (int i = 0; i < V; i++) v[i] = OP::value(k, sh.slope, a[i], d[i]);
+        for (int j = 0; j < V; j++) v[j] = OP::value(k, sh.slope, a.at(j), OP::kTwo ? d.at(j) : 0.f);
         store<T, V>(po + e, v);
     }
 #pragma unroll
-    for (int i = 0; i < V; i++)
-        if (e + i < hi) po[e + i] = (R)OP::value(k, sh.slope, (float)px[e + i], OP::kTwo ? (float)pd[e + i] : 0.f);
+    for (int j = 0; j < V; j++)
+        if (e + j < hi) po[e + j] = (R)OP::value(k, sh.slope, (float)px[e + j], OP::kTwo ? (float)pd[e + j] : 0.f);
 }
 
-// ---- between the passes -----------------------------------------------------------------------------------------
-// one workgroup per image and group: the chunks' sums -> mean and 1 / sqrt(var + eps)
+// ---- between the passes, where the second does not do it: one workgroup per image and group ---------------------
 template <class T>
-__global__ __launch_bounds__(256) void stats_kernel(Map x, Shape sh, int chunks, const double2 *part, double *stats)
+__global__ __launch_bounds__(256) void stats_kernel(Map x, Shape sh, Between bt)
 {
-    __shared__ double lds[16];
+    __shared__ double lds[32];
     const int n = blockIdx.x / sh.G, g = blockIdx.x % sh.G;
-    const double2 *p = part + (int64_t)n * chunks * sh.C + g * sh.cg;
-    double s = 0, q = 0;
-    for (int64_t i = threadIdx.x; i < (int64_t)chunks * sh.cg; i += blockDim.x) {
-        const double2 v = p[i / sh.cg * sh.C + i % sh.cg];
-        s += v.x;
-        q += v.y;
-    }
-    s = block_sum(s, lds);
-    q = block_sum(q, lds);
-    if (threadIdx.x == 0) {
-        const double d = s / sh.m, var = fma(-d, d, q / sh.m);
-        stats[blockIdx.x] = first_value<T>(x, sh, n, g) + d;                // (equal values: the mean is theirs, exactly)
-        stats[sh.N * sh.G + blockIdx.x] = 1. / sqrt((var < 0 ? 0. : var) + sh.eps);      // (a NaN stays one)
-    }
+    const double2 t = group_total<false>(sh, bt.chunks, bt.chan, n, g, nullptr, 0, lds);
+    if (threadIdx.x == 0) keep_stat(sh, bt.stats, blockIdx.x, stat_of<T>(x, sh, n, g, t.x, t.y));
 }
-
-// one workgroup per image and group: the chunks' sums -> per channel (for dw, db) and, weighted, per group (m1, m2)
-__global__ __launch_bounds__(256) void group_sums_kernel(Shape sh, int chunks, const double2 *part, const double *stats, const void *w, int wt, double2 *chan, double *sums)
+__global__ __launch_bounds__(256) void group_sums_kernel(Shape sh, Between bt, const void *w, int wt, double *sums)
 {
-    __shared__ double lds[16];
-    __shared__ double2 team[256];
+    __shared__ double lds[32];
     const int n = blockIdx.x / sh.G, g = blockIdx.x % sh.G;
-    int lanes = 1;                                                         // threads of a team that add one channel's chunks
-    while (lanes * 2 * sh.cg <= 256 && lanes < chunks) lanes *= 2;
-    const int teams = 256 / lanes, l = threadIdx.x % lanes, first = threadIdx.x / lanes;
-    const double r = stats[sh.N * sh.G + blockIdx.x];
-    double m1 = 0, m2 = 0;
-    for (int j0 = 0; j0 < sh.cg; j0 += teams) {
-        const int j = j0 + first, c = g * sh.cg + j;
-        double2 v = make_double2(0, 0);
-        if (j < sh.cg)
-            for (int i = l; i < chunks; i += lanes) {
-                const double2 u = part[((int64_t)n * chunks + i) * sh.C + c];
-                v.x += u.x;
-                v.y += u.y;
-            }
-        __syncthreads();
-        team[threadIdx.x] = v;
-        __syncthreads();
-        if (l == 0 && j < sh.cg) {
-            for (int i = 1; i < lanes; i++) {
-                v.x += team[threadIdx.x + i].x;
-                v.y += team[threadIdx.x + i].y;
-            }
-            v.y *= r;                                                      // sum dz h
-            chan[(int64_t)n * sh.C + c] = v;
-            const double wc = load_param(w, wt, c, 1.f);
-            m1 = fma(wc, v.x, m1);
-            m2 = fma(wc, v.y, m2);
-        }
-    }
-    m1 = block_sum(m1, lds);
-    m2 = block_sum(m2, lds);
+    const double2 t = group_total<true>(sh, bt.chunks, bt.chan, n, g, w, wt, lds);
     if (threadIdx.x == 0) {
-        sums[2 * blockIdx.x] = m1 / sh.m;
-        sums[2 * blockIdx.x + 1] = m2 / sh.m;
+        sums[2 * blockIdx.x] = t.x / sh.m;
+        sums[2 * blockIdx.x + 1] = t.y * bt.stats[sh.N * sh.G + blockIdx.x] / sh.m;      // sum w dz h / M
     }
 }
 
@@ -348,20 +467,30 @@ inline bool channels_first(const genre_tensor *t) { return t->size[2] == 1 || t-
 inline bool gapless(const genre_tensor *t) { return t->size[2] == 1 || t->stride[2] == t->size[1]; }
 inline Map map_of(const genre_tensor *t) { return {t->data, t->stride[0], t->stride[1], t->size[2] == 1 ? t->size[1] : t->stride[2]}; }
 
-constexpr int kWorkgroups = 2048;                                          // eight of 256 threads for each CU
-
 // values per thread and access: 16 bytes; fewer only where a channels-last column may not cross a row's end
 int width_of(const genre_tensor *x, bool last, bool dense)
 {
     int v = x->dtype == GENRE_F32 ? 4 : 8;
     if (last) {
         const int C = (int)x->size[1];
-        if (!dense || C / gcd(C, v) > 512) v = gcd(C, v);
+        if (!dense || C > 1024 || C / gcd(C, v) > 512) v = gcd(C, v);   // (a period's coefficients and columns have to fit a workgroup)
     }
     return v;
 }
 
-Cut cut_of(int N, int C, int64_t S, int v)
+// Workgroups: as many as the chip holds of a pass (the sums' need more registers and end with a reduction), and four accesses a
+// thread at least.
+constexpr int kSumsWorkgroups = 1024, kValueWorkgroups = 2048;
+constexpr int kJoined = 1024;                                              // pairs that a workgroup of the second pass adds up itself
+
+int chunks_of(int64_t turns, int64_t others, int workgroups, int64_t most)
+{
+    const int64_t fill = (workgroups + others - 1) / others, few = (turns + kBatch - 1) / kBatch;
+    const int64_t c = few < fill ? few : fill;
+    return (int)(c < most ? c : most);
+}
+
+Cut cut_of(int N, int C, int64_t S, int v, int workgroups, int64_t most, int *threads)
 {
     Cut c;
     const int g = gcd(C, v);
@@ -369,36 +498,59 @@ Cut cut_of(int N, int C, int64_t S, int v)
     c.cols = C / g;
     c.tiles = ceil_div(c.cols, 512);
     c.tile = ceil_div(c.cols, c.tiles);
-    const int want = c.tile > 256 ? 512 : 256;
-    c.deep = want / c.tile;
-    c.threads = (c.deep * c.tile + 63) / 64 * 64;
+    c.deep = (c.tile > 256 ? 512 : 256) / c.tile;
+    *threads = (c.deep * c.tile + 63) / 64 * 64;
     c.periods = (S + c.rows - 1) / c.rows;
-    // four accesses a thread at least, then as many workgroups as fill the chip
-    const int64_t turns = (c.periods + c.deep - 1) / c.deep, most = (turns + 3) / 4, fill = (kWorkgroups + (int64_t)N * c.tiles - 1) / ((int64_t)N * c.tiles);
-    const int64_t chunks = most < fill ? most : fill;
+    const int64_t turns = (c.periods + c.deep - 1) / c.deep;
+    const int chunks = chunks_of(turns, (int64_t)N * c.tiles, workgroups, most);
     c.per = (turns + chunks - 1) / chunks * c.deep;
     c.chunks = (int)((c.periods + c.per - 1) / c.per);
     return c;
 }
 
-void first_cut(int N, int C, int64_t S, int v, int *threads, int *chunks, int64_t *per)
+Run run_of(int N, int C, int64_t S, int v, int threads, int workgroups, int64_t most)
 {
-    *threads = S <= 64 * v * 4 ? 64 : 256;
-    const int64_t step = (int64_t)*threads * v, turns = (S + step - 1) / step, most = (turns + 3) / 4;
-    const int64_t fill = (kWorkgroups + (int64_t)N * C - 1) / ((int64_t)N * C), want = most < fill ? most : fill;
-    *per = (turns + want - 1) / want * step;
-    *chunks = (int)((S + *per - 1) / *per);
+    const int64_t step = (int64_t)threads * v, turns = (S + step - 1) / step;
+    const int chunks = chunks_of(turns, (int64_t)N * C, workgroups, most);
+    const int64_t per = (turns + chunks - 1) / chunks * step;
+    return {per, (int)((S + per - 1) / per)};
 }
 
 struct Call {
     Shape sh;
-    bool last;
-    int v;
-    Cut cut;
-    int threads, chunks;
-    int64_t per;
-    int64_t blocks() const { return (int64_t)sh.N * (last ? cut.tiles : sh.C) * chunks; }
+    bool last, joined;
+    int v, threads;
+    Cut sums, values;                                                      // channels last
+    Run rsums, rvalues;                                                    // channels first
+    int chunks() const { return last ? sums.chunks : rsums.chunks; }
+    int64_t sums_blocks() const { return (int64_t)sh.N * (last ? sums.tiles : sh.C) * chunks(); }
+    int64_t value_blocks() const { return (int64_t)sh.N * (last ? values.tiles * (int64_t)values.chunks : sh.C * (int64_t)rvalues.chunks); }
+    size_t sums_lds(size_t coef) const
+    {
+        const size_t a = sizeof(double2) * v * threads + (joined ? sizeof(double2) * sh.C : 0), b = coef_bytes(sh, sums, v, coef);
+        return a > b ? a : b;
+    }
 };
+
+void cut_call(Call &c, int64_t N, int64_t C, int64_t S, int groups)
+{
+    if (c.last) {
+        // the second pass joins the sums where few enough chunks fill half the chip, and a workgroup sees all channels
+        const int64_t most = kJoined / groups;
+        c.sums = cut_of((int)N, (int)C, S, c.v, kSumsWorkgroups, INT32_MAX, &c.threads);
+        c.joined = c.sums.tiles == 1 && groups <= kJoinedGroups && C <= 512 && c.threads * c.v <= 2048 &&
+                   (c.sums.chunks <= most || N * most >= kSumsWorkgroups / 2);
+        if (c.joined) c.sums = cut_of((int)N, (int)C, S, c.v, kSumsWorkgroups, most, &c.threads);
+        c.values = cut_of((int)N, (int)C, S, c.v, kValueWorkgroups, INT32_MAX, &c.threads);
+    } else {
+        c.threads = S <= 64 * c.v * 4 ? 64 : 256;
+        const int64_t cg = C / groups, most = kJoined / cg;
+        c.rsums = run_of((int)N, (int)C, S, c.v, c.threads, kSumsWorkgroups, INT32_MAX);
+        c.joined = c.rsums.chunks <= most || (most > 0 && N * C * most >= kSumsWorkgroups / 2);
+        if (c.joined) c.rsums = run_of((int)N, (int)C, S, c.v, c.threads, kSumsWorkgroups, most);
+        c.rvalues = run_of((int)N, (int)C, S, c.v, c.threads, kValueWorkgroups, INT32_MAX);
+    }
+}
 
 int plan(const char *op, const genre_tensor *x, const genre_tensor *const *others, int n_others, int groups, Call &c)
 {
@@ -418,86 +570,95 @@ int plan(const char *op, const genre_tensor *x, const genre_tensor *const *other
     c.v = width_of(x, last, dense);
     if (N * S == 0) return 1;
     c.sh.m = (double)(C / groups) * (double)S;
-    if (last) {
-        c.cut = cut_of((int)N, (int)C, S, c.v);
-        c.chunks = c.cut.chunks;
-        c.threads = c.cut.threads;
-    } else {
-        first_cut((int)N, (int)C, S, c.v, &c.threads, &c.chunks, &c.per);
-    }
-    GENRE_REQUIRE(c.blocks() < INT32_MAX && N * groups < INT32_MAX, "%s: the map is too large for one launch", op);
+    cut_call(c, N, C, S, groups);
+    GENRE_REQUIRE(c.sums_blocks() < INT32_MAX && c.value_blocks() + C < INT32_MAX && N * (int64_t)c.chunks() < INT32_MAX && N * groups < INT32_MAX / 2 &&
+                      c.chunks() * (C / groups) < INT32_MAX,
+                  "%s: the map is too large for one launch", op);
     return 1;
 }
 
-// fp64 values of the workspace: the chunks' sums; backward: and those per image and channel, per image and group
+// fp64 values of the workspace: the chunks' sums by channel (forward: unless they are joined by group), by group, the groups'
+int64_t chan_values(const Call &c, bool backward) { return backward || !(c.last && c.joined) ? 2 * (int64_t)c.sh.N * c.sh.C * c.chunks() : 0; }
+int64_t group_values(const Call &c) { return c.last && c.joined ? 2 * (int64_t)c.sh.N * c.sh.G * c.chunks() : 0; }
 int64_t workspace_of(const Call &c, bool backward)
 {
-    const int64_t chan = (int64_t)c.sh.N * c.sh.C;
-    return 2 * chan * c.chunks + (backward ? 2 * chan + 2 * (int64_t)c.sh.N * c.sh.G : 0);
+    return chan_values(c, backward) + group_values(c) + (backward && !c.joined ? 2 * (int64_t)c.sh.N * c.sh.G : 0);
 }
 
 int check_f64(const char *op, const char *what, const genre_tensor *t, int64_t least)
 {
     if (least == 0) return 1;
-    GENRE_REQUIRE(t && t->data && t->dtype == GENRE_F64 && is_contiguous(t) && numel(t) >= least,
-                  "%s: %s must be a contiguous fp64 tensor of at least %lld values", op, what, (long long)least);
+    GENRE_REQUIRE(t && t->data && t->dtype == GENRE_F64 && is_contiguous(t) && numel(t) >= least && aligned16(t->data),
+                  "%s: %s must be a contiguous fp64 tensor of at least %lld values, on a multiple of 16 bytes", op, what, (long long)least);
     return 1;
 }
 
-template <class T, int V, class OP>
-void sums(const Call &c, const Map &x, const Map &dy, const Params &p, const double *stats, double2 *part, hipStream_t st)
+struct Space { double2 *chan, *group; double *sums; };
+Space space_of(const Call &c, bool backward, double *ws)
 {
-    if (c.last)
-        last_sums_kernel<T, V, OP><<<(int)c.blocks(), c.threads, sizeof(double) * 2 * V * c.threads, st>>>(x, dy, c.sh, c.cut, stats, p.w, p.b, p.wt, p.bt, part);
-    else if constexpr (V * sizeof(typename T::raw) == 16)                  // (width_of narrows channels-last columns only)
-        first_sums_kernel<T, V, OP><<<(int)c.blocks(), c.threads, 0, st>>>(x, dy, c.sh, c.chunks, c.per, stats, p.w, p.b, p.wt, p.bt, part);
+    const int64_t chan = chan_values(c, backward), group = group_values(c);
+    return {chan ? (double2 *)ws : nullptr, group ? (double2 *)(ws + chan) : nullptr, ws + chan + group};
+}
+
+template <class T, int V, class OP>
+int sums(const Call &c, const Map &x, const Map &dy, const Params &p, const Between &k, const Space &to, hipStream_t st)
+{
+    if (c.last) {
+        const size_t lds = c.sums_lds(sizeof(typename OP::Coef));
+        last_sums_kernel<T, V, OP><<<(int)c.sums_blocks(), c.threads, lds, st>>>(x, dy, c.sh, c.sums, k, p.w, p.b, p.wt, p.bt, to.chan, to.group);
+    } else if constexpr (V * sizeof(typename T::raw) == 16) {              // (width_of narrows channels-last columns only)
+        first_sums_kernel<T, V, OP><<<(int)c.sums_blocks(), c.threads, 0, st>>>(x, dy, c.sh, c.rsums, k, p.w, p.b, p.wt, p.bt, to.chan);
+    }
+    GENRE_LAUNCH_CHECK("group norm sums");
+    return 1;
 }
 template <class T, int V, class OP>
-void values(const Call &c, const Map &x, const Map &dy, const Map &out, const Params &p, const double *stats, const double *sm, hipStream_t st)
+int values(const Call &c, const Map &x, const Map &dy, const Map &out, const Params &p, const Between &k, hipStream_t st)
 {
+    const int blocks = (int)k.blocks + (k.dw || k.db ? ceil_div(c.sh.C, c.threads / 64) : 0);
     if (c.last)
-        last_value_kernel<T, V, OP><<<(int)c.blocks(), c.threads, 0, st>>>(x, dy, out, c.sh, c.cut, stats, sm, p.w, p.b, p.wt, p.bt);
+        last_value_kernel<T, V, OP><<<blocks, c.threads, coef_bytes(c.sh, c.values, V, sizeof(typename OP::Coef)), st>>>(x, dy, out, c.sh, c.values, k, p.w, p.b, p.wt, p.bt);
     else if constexpr (V * sizeof(typename T::raw) == 16)
-        first_value_kernel<T, V, OP><<<(int)c.blocks(), c.threads, 0, st>>>(x, dy, out, c.sh, c.chunks, c.per, stats, sm, p.w, p.b, p.wt, p.bt);
+        first_value_kernel<T, V, OP><<<blocks, c.threads, 0, st>>>(x, dy, out, c.sh, c.rvalues, k, p.w, p.b, p.wt, p.bt);
+    GENRE_LAUNCH_CHECK("group norm values");
+    return 1;
 }
 
 template <class T, int V>
 int forward(const Call &c, const Map &x, const Map &y, const Params &p, double *stats, double *ws, hipStream_t st)
 {
-    double2 *part = (double2 *)ws;
-    sums<T, V, SumsF<T>>(c, x, Map{}, p, stats, part, st);
-    GENRE_LAUNCH_CHECK("group norm sums");
-    stats_kernel<T><<<c.sh.N * c.sh.G, 256, 0, st>>>(x, c.sh, c.chunks, part, stats);
-    GENRE_LAUNCH_CHECK("group norm statistics");
-    switch (c.sh.act) {
-    case kActRelu: values<T, V, ValueF<T, kActRelu>>(c, x, Map{}, y, p, stats, nullptr, st); break;
-    case kActLeaky: values<T, V, ValueF<T, kActLeaky>>(c, x, Map{}, y, p, stats, nullptr, st); break;
-    case kActSilu: values<T, V, ValueF<T, kActSilu>>(c, x, Map{}, y, p, stats, nullptr, st); break;
-    default: values<T, V, ValueF<T, kActNone>>(c, x, Map{}, y, p, stats, nullptr, st); break;
+    const Space to = space_of(c, false, ws);
+    const Between k = {c.joined, c.chunks(), to.chan, to.group, stats, nullptr, nullptr, nullptr, 0, 0, (unsigned)c.value_blocks()};
+    if (!sums<T, V, SumsF<T>>(c, x, Map{}, p, k, to, st)) return 0;
+    if (!c.joined) {
+        stats_kernel<T><<<c.sh.N * c.sh.G, 256, 0, st>>>(x, c.sh, k);
+        GENRE_LAUNCH_CHECK("group norm statistics");
     }
-    GENRE_LAUNCH_CHECK("group norm values");
-    return 1;
+    switch (c.sh.act) {
+    case kActRelu: return values<T, V, ValueF<T, kActRelu>>(c, x, Map{}, y, p, k, st);
+    case kActLeaky: return values<T, V, ValueF<T, kActLeaky>>(c, x, Map{}, y, p, k, st);
+    case kActSilu: return values<T, V, ValueF<T, kActSilu>>(c, x, Map{}, y, p, k, st);
+    default: return values<T, V, ValueF<T, kActNone>>(c, x, Map{}, y, p, k, st);
+    }
 }
 
 template <class T, int V, int ACT>
 int backward_as(const Call &c, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
 {
-    const int64_t nc = (int64_t)c.sh.N * c.sh.C;
-    double2 *part = (double2 *)ws, *chan = part + nc * c.chunks;
-    double *sm = (double *)(chan + nc);
-    sums<T, V, SumsB<T, ACT>>(c, x, dy, p, stats, part, st);
-    GENRE_LAUNCH_CHECK("group norm backward sums");
-    group_sums_kernel<<<c.sh.N * c.sh.G, 256, 0, st>>>(c.sh, c.chunks, part, stats, p.w, p.wt, chan, sm);
-    GENRE_LAUNCH_CHECK("group norm backward group sums");
-    if (g.dw || g.db) {
-        param_grads_kernel<<<ceil_div(c.sh.C, 256), 256, 0, st>>>(c.sh, chan, g.dw, g.dwt, g.db, g.dbt);
+    const Space to = space_of(c, true, ws);
+    const Between k = {c.joined, c.chunks(), to.chan, to.group, (double *)stats, to.sums, g.dw, g.db, g.dwt, g.dbt, (unsigned)c.value_blocks()};
+    if (!sums<T, V, SumsB<T, ACT>>(c, x, dy, p, k, to, st)) return 0;
+    if (!g.dx.p) {
+        if (!g.dw && !g.db) return 1;
+        channel_grads_kernel<<<ceil_div(c.sh.C, 4), 256, 0, st>>>(c.sh, k.chunks, k.chan, stats, g.dw, g.dwt, g.db, g.dbt);
         GENRE_LAUNCH_CHECK("group norm parameter gradients");
+        return 1;
     }
-    if (g.dx.p) {
-        values<T, V, ValueB<T, ACT>>(c, x, dy, g.dx, p, stats, sm, st);
-        GENRE_LAUNCH_CHECK("group norm input gradient");
+    if (!c.joined) {
+        group_sums_kernel<<<c.sh.N * c.sh.G, 256, 0, st>>>(c.sh, k, p.w, p.wt, to.sums);
+        GENRE_LAUNCH_CHECK("group norm backward group sums");
     }
-    return 1;
+    return values<T, V, ValueB<T, ACT>>(c, x, dy, g.dx, p, k, st);
 }
 template <class T, int V>
 int backward(const Call &c, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
@@ -529,8 +690,7 @@ extern "C" int64_t genre_group_norm_workspace(const genre_tensor *x, int groups,
     if (c.last) {                                                          // a gap in another map's rows narrows the columns: room for both
         Call d = c;
         d.v = width_of(x, true, false);
-        d.cut = cut_of(c.sh.N, c.sh.C, c.sh.S, d.v);
-        d.chunks = d.cut.chunks;
+        cut_call(d, d.sh.N, d.sh.C, d.sh.S, groups);
         const int64_t other = workspace_of(d, backward != 0);
         if (other > need) need = other;
     }
@@ -591,7 +751,7 @@ extern "C" int genre_group_norm_backward(const genre_tensor *x, const genre_tens
         if (g.dw || g.db) {
             Shape none = c.sh;
             none.N = 0;
-            param_grads_kernel<<<ceil_div(none.C, 256), 256, 0, st>>>(none, nullptr, g.dw, g.dwt, g.db, g.dbt);
+            channel_grads_kernel<<<ceil_div(none.C, 4), 256, 0, st>>>(none, 1, nullptr, nullptr, g.dw, g.dwt, g.db, g.dbt);
             GENRE_LAUNCH_CHECK("group norm parameter gradients");
         }
         return 1;

@@ -2,6 +2,7 @@
 // kernels that walk a map in several passes; group_norm_small.hip: one workgroup per image and group).
 #pragma once
 #include "common.hpp"
+#include <type_traits>
 
 namespace genre {
 namespace gn {
@@ -13,15 +14,6 @@ struct F32 { using raw = float; };
 struct F16 { using raw = _Float16; };
 struct BF16 { using raw = __bf16; };
 
-// V values of type T; the pointer needs no more than T's own alignment (gfx950 loads and stores 16 bytes at any address)
-template <class T, int V>
-__device__ __forceinline__ void load(const typename T::raw *p, float (&v)[V])
-{
-    typename T::raw t[V];
-    __builtin_memcpy(t, p, sizeof(t));
-#pragma unroll
-    for (int i = 0; i < V; i++) v[i] = (float)t[i];
-}
 template <class T, int V>
 __device__ __forceinline__ void store(typename T::raw *p, const float (&v)[V])
 {
@@ -30,6 +22,32 @@ __device__ __forceinline__ void store(typename T::raw *p, const float (&v)[V])
     for (int i = 0; i < V; i++) t[i] = (typename T::raw)v[i];              // round to nearest even
     __builtin_memcpy(p, t, sizeof(t));
 }
+
+// Loads and stores of V values need no more than their type's own alignment (gfx950 moves 16 bytes at any address).
+// V values as they lie in memory: a thread keeps these, two 16-bit values to a register, and converts them in each pass
+template <class T, int V>
+struct Kept {
+    static constexpr int kWords = (V * sizeof(typename T::raw) + 3) / 4;
+    unsigned word[kWords];
+    __device__ void load(const typename T::raw *p)
+    {
+        if (V * sizeof(*p) == 2) word[0] = *(const unsigned short *)p;
+        else __builtin_memcpy(word, p, V * sizeof(*p));
+    }
+    __device__ float at(int i) const
+    {
+        if (sizeof(typename T::raw) == 4) return __uint_as_float(word[i]);
+        const unsigned short h = (unsigned short)(word[i / 2] >> (i % 2 * 16));
+        return (float)__builtin_bit_cast(half_of, h);
+    }
+    // the conversions of one pass are not kept for the next (fp64: two registers a value)
+    __device__ void fresh()
+    {
+#pragma unroll
+        for (int i = 0; i < kWords; i++) asm volatile("" : "+v"(word[i]));
+    }
+    typedef typename std::conditional<sizeof(typename T::raw) == 2, typename T::raw, _Float16>::type half_of;
+};
 
 __device__ __forceinline__ float load_param(const void *p, int dtype, int c, float missing)
 {
@@ -86,20 +104,7 @@ __device__ __forceinline__ double wave_sum(double v)
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
-// sum over the workgroup, in every thread; `lds` has 16 doubles; ends with a barrier before lds can be used again
-__device__ __forceinline__ double block_sum(double v, double *lds)
-{
-    v = wave_sum(v);
-    const int waves = (blockDim.x + 63) / 64;
-    __syncthreads();
-    if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = v;
-    __syncthreads();
-    double s = 0;
-    for (int i = 0; i < waves; i++) s += lds[i];
-    return s;
-}
-
-// two of them at once; `lds` has 32
+// sums over the workgroup of two values, in every thread; `lds` has 32 doubles (blockDim.x <= 1024)
 __device__ __forceinline__ void block_sum2(double &a, double &b, double *lds)
 {
     a = wave_sum(a);
@@ -129,19 +134,27 @@ __device__ __forceinline__ double first_value(const Map &x, const Shape &sh, int
 }
 
 
-// dw and db from the sums of dz and dz h of each image and channel, whatever order the images' workgroups ended in
-static __global__ __launch_bounds__(256) void param_grads_kernel(Shape sh, const double2 *chan, void *dw, int wt, void *db, int bt)
+// The chunks' sums lie in the workspace as double2 [image][chunk][channel] of dz and dz (x - mean) (one chunk: an image's).
+// dw and db of one channel from them, by one wave: in this order whatever order the workgroups that left them ended in.
+__device__ __forceinline__ void channel_grads(const Shape &sh, int chunks, const double2 *part, const double *stats, int c, void *dw, int wt, void *db, int bt)
 {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= sh.C) return;
     double a = 0, b = 0;
-    for (int n = 0; n < sh.N; n++) {
-        const double2 v = chan[(int64_t)n * sh.C + c];
+    const unsigned rows = (unsigned)sh.N * chunks;
+    for (unsigned i = threadIdx.x % 64; i < rows; i += 64) {
+        const double2 v = part[(int64_t)i * sh.C + c];
         a += v.x;
-        b += v.y;
+        b = fma(v.y, stats[(unsigned)sh.N * sh.G + i / (unsigned)chunks * sh.G + c / sh.cg], b);
     }
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if (threadIdx.x % 64) return;
     if (db) store_param(db, bt, c, a);
     if (dw) store_param(dw, wt, c, b);
+}
+static __global__ __launch_bounds__(256) void channel_grads_kernel(Shape sh, int chunks, const double2 *part, const double *stats, void *dw, int wt, void *db, int bt)
+{
+    const int c = blockIdx.x * 4 + threadIdx.x / 64;
+    if (c < sh.C) channel_grads(sh, chunks, part, stats, c, dw, wt, db, bt);
 }
 
 inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }

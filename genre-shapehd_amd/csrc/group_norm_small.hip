@@ -4,7 +4,6 @@
 // scratch.  A group is `rows` runs of `cols` accesses of V values: channels last, a run is one position's cg channels and every
 // thread keeps one column; channels first, a run is one channel's positions, shared by a team of 2^k threads.
 #include "group_norm.hpp"
-#include <type_traits>
 
 namespace genre {
 namespace {
@@ -43,31 +42,6 @@ __device__ __forceinline__ int by_die(int b, int n)
     const int die = b & 7, each = n >> 3, more = n & 7;
     return die * each + min(die, more) + (b >> 3);
 }
-
-// V values as they lie in memory: a thread keeps these, two 16-bit values to a register, and converts them in each pass
-template <class T, int V>
-struct Kept {
-    static constexpr int kWords = (V * sizeof(typename T::raw) + 3) / 4;
-    unsigned word[kWords];
-    __device__ void load(const typename T::raw *p)
-    {
-        if (V * sizeof(*p) == 2) word[0] = *(const unsigned short *)p;
-        else __builtin_memcpy(word, p, V * sizeof(*p));
-    }
-    __device__ float at(int i) const
-    {
-        if (sizeof(typename T::raw) == 4) return __uint_as_float(word[i]);
-        const unsigned short h = (unsigned short)(word[i / 2] >> (i % 2 * 16));
-        return (float)__builtin_bit_cast(half_of, h);
-    }
-    // the conversions of one pass are not kept for the next (fp64: two registers a value)
-    __device__ void fresh()
-    {
-#pragma unroll
-        for (int i = 0; i < kWords; i++) asm volatile("" : "+v"(word[i]));
-    }
-    typedef typename std::conditional<sizeof(typename T::raw) == 2, typename T::raw, _Float16>::type half_of;
-};
 
 // a thread's accesses, one after the other: run, column (in accesses), and whether there is one
 template <bool LAST>
@@ -153,7 +127,7 @@ __global__ __launch_bounds__(1024) void small_forward_kernel(Map x, Map y, Shape
     }
 }
 
-// chan: the sums of dz and dz h by image and channel (more than one image: added up behind this), or dw and db themselves
+// chan: the sums of dz and dz (x - mean) by image and channel (more than one image: added up behind this), or dw and db themselves
 template <class T, int V, int K, bool LAST>
 __global__ __launch_bounds__(512) void small_backward_kernel(Map x, Map dy, Map dx, Shape sh, Small m, const double *stats, const void *w, const void *b, int wt,
                                                              int bt, double2 *chan, void *dw, void *db)
@@ -241,8 +215,8 @@ __global__ __launch_bounds__(512) void small_backward_kernel(Map x, Map dy, Map 
                 a.y += scratch[c * m.subs + i].y;
             }
         }
-        a.y *= r;
         if (chan) chan[(int64_t)n * sh.C + g * cg + c] = a;
+        a.y *= r;
         if (db) store_param(db, bt, g * cg + c, a.x);
         if (dw) store_param(dw, wt, g * cg + c, a.y);
         m1 = fma(coef[2 * cg + c], a.x, m1);
@@ -343,7 +317,7 @@ int backward_k(const Shape &sh, const SmallCall &k, const Map &x, const Map &dy,
     small_backward_kernel<T, V, K, LAST><<<sh.N * sh.G, k.threads, lds, st>>>(x, dy, g.dx, sh, k.m, stats, p.w, p.b, p.wt, p.bt, chan, one ? g.dw : nullptr, one ? g.db : nullptr);
     GENRE_LAUNCH_CHECK("group norm backward");
     if (chan) {
-        param_grads_kernel<<<ceil_div(sh.C, 256), 256, 0, st>>>(sh, chan, g.dw, g.dwt, g.db, g.dbt);
+        channel_grads_kernel<<<ceil_div(sh.C, 4), 256, 0, st>>>(sh, 1, chan, stats, g.dw, g.dwt, g.db, g.dbt);
         GENRE_LAUNCH_CHECK("group norm parameter gradients");
     }
     return 1;

@@ -114,6 +114,8 @@ SHAPES = [
     # groups of more values than one workgroup holds (65536 forward, 32768 backward), of more channels, and at the border
     (2, 45, 1, (41, 40)), (1, 511, 1, (13, 11)), (1, 1030, 2, (9, 15)), (1, 1030, 1, (3,)), (1, 4104, 2, (5, 7)), (2, 7, 1, (101, 97)), (1, 3, 1, (40001,)),
     (1, 64, 2, (32, 32)), (1, 64, 2, (32, 33)), (1, 64, 1, (32, 32)), (1, 64, 1, (32, 33)), (1, 96, 1, (700,)),
+    # more groups or channels than a second pass adds up itself; columns that run over a row's end; one channel
+    (1, 40, 8, (64, 64, 20)), (1, 1500, 1, (40,)), (1, 45, 5, (91, 93)), (1, 1001, 1, (7, 5, 2)), (1, 300, 1, (15, 16)), (2, 1, 1, (257, 259)), (3, 65, 65, (210, 160)),
 ]
 
 
