@@ -322,7 +322,7 @@ __global__ __launch_bounds__(512) void last_value_kernel(Map x, Map dy, Map out,
         if (OP::kTwo) d.load(pd + p * dd);
 #pragma unroll
         for (int i = 0; i < V; i++) v[i] = OP::value(k[i], sh.slope, a.at(i), OP::kTwo ? d.at(i) : 0.f);
-        store<T, V>(po + p * dout, v);
+        store<T, V, true>(po + p * dout, v);
     }
     if (p < hi) {
         const int64_t left = (sh.S - p * cut.rows) * sh.C - col * V;
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(256) void first_value_kernel(Map x, Map dy, Map out
         if (OP::kTwo) d.load(pd + e);
 #pragma unroll
         for (int j = 0; j < V; j++) v[j] = OP::value(k, sh.slope, a.at(j), OP::kTwo ? d.at(j) : 0.f);
-        store<T, V>(po + e, v);
+        store<T, V, true>(po + e, v);
     }
 #pragma unroll
     for (int j = 0; j < V; j++)
@@ -478,9 +478,11 @@ int width_of(const genre_tensor *x, bool last, bool dense)
     return v;
 }
 
-// Workgroups: as many as the chip holds of a pass (the sums' need more registers and end with a reduction), and four accesses a
-// thread at least.
-constexpr int kSumsWorkgroups = 1024, kValueWorkgroups = 2048;
+// Workgroups, with four accesses a thread at least.  Sums 1024 / 2048: refiner 64^3 x4, channels last, whose workgroups end with a
+// reduction by column, 47.4 / 51.3 us (training 126 / 137); decoder 64^3 x8, channels first, 73.5 / 71.3 (179 / 175).  Values 2048 /
+// 4096: 47.4 / 47.4 and 73.5 / 72.0 (126.1 / 125.9 and 179.5 / 177.2).
+constexpr int kSumsLast = 1024, kSumsFirst = 2048, kValueWorkgroups = 4096;
+constexpr int kFew = 32;
 constexpr int kJoined = 1024;                                              // pairs that a workgroup of the second pass adds up itself
 
 int chunks_of(int64_t turns, int64_t others, int workgroups, int64_t most)
@@ -535,19 +537,22 @@ struct Call {
 void cut_call(Call &c, int64_t N, int64_t C, int64_t S, int groups)
 {
     if (c.last) {
-        // the second pass joins the sums where few enough chunks fill half the chip, and a workgroup sees all channels
+        // the second pass joins the sums where few enough chunks fill half the chip or have few accesses each, and a workgroup sees
+        // all channels
         const int64_t most = kJoined / groups;
-        c.sums = cut_of((int)N, (int)C, S, c.v, kSumsWorkgroups, INT32_MAX, &c.threads);
+        c.sums = cut_of((int)N, (int)C, S, c.v, kSumsLast, INT32_MAX, &c.threads);
+        const int64_t turns = (c.sums.periods + c.sums.deep - 1) / c.sums.deep;
         c.joined = c.sums.tiles == 1 && groups <= kJoinedGroups && C <= 512 && c.threads * c.v <= 2048 &&
-                   (c.sums.chunks <= most || N * most >= kSumsWorkgroups / 2);
-        if (c.joined) c.sums = cut_of((int)N, (int)C, S, c.v, kSumsWorkgroups, most, &c.threads);
+                   (c.sums.chunks <= most || N * most >= kSumsLast / 2 || turns <= kFew * most);
+        if (c.joined) c.sums = cut_of((int)N, (int)C, S, c.v, kSumsLast, most, &c.threads);
         c.values = cut_of((int)N, (int)C, S, c.v, kValueWorkgroups, INT32_MAX, &c.threads);
     } else {
         c.threads = S <= 64 * c.v * 4 ? 64 : 256;
         const int64_t cg = C / groups, most = kJoined / cg;
-        c.rsums = run_of((int)N, (int)C, S, c.v, c.threads, kSumsWorkgroups, INT32_MAX);
-        c.joined = c.rsums.chunks <= most || (most > 0 && N * C * most >= kSumsWorkgroups / 2);
-        if (c.joined) c.rsums = run_of((int)N, (int)C, S, c.v, c.threads, kSumsWorkgroups, most);
+        c.rsums = run_of((int)N, (int)C, S, c.v, c.threads, kSumsFirst, INT32_MAX);
+        const int64_t turns = (S + c.threads * c.v - 1) / (c.threads * c.v);
+        c.joined = c.rsums.chunks <= most || (most > 0 && (N * C * most >= kSumsFirst / 2 || turns <= kFew * most));
+        if (c.joined) c.rsums = run_of((int)N, (int)C, S, c.v, c.threads, kSumsFirst, most);
         c.rvalues = run_of((int)N, (int)C, S, c.v, c.threads, kValueWorkgroups, INT32_MAX);
     }
 }
@@ -685,7 +690,7 @@ extern "C" int64_t genre_group_norm_workspace(const genre_tensor *x, int groups,
     if (!x) { fail("%s: x is NULL", op); return -1; }
     if (!check_map(op, "x", x, x) || !plan(op, x, nullptr, 0, groups, c)) return -1;
     if (numel(x) == 0) return 0;
-    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, backward != 0)) return backward ? small_workspace(c.sh) : 0;
+    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2)) return backward ? small_workspace(c.sh) : 0;
     int64_t need = workspace_of(c, backward != 0);
     if (c.last) {                                                          // a gap in another map's rows narrows the columns: room for both
         Call d = c;
@@ -718,7 +723,7 @@ extern "C" int genre_group_norm_forward(const genre_tensor *x, const genre_tenso
     const Map mx = map_of(x), my = map_of(y);
     double *s = (double *)stats->data;
     hipStream_t st = (hipStream_t)stream;
-    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, false)) return small_forward(c.last, x->dtype, c.sh, mx, my, p, s, st);
+    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2)) return small_forward(c.last, x->dtype, c.sh, mx, my, p, s, st);
     if (!check_f64(op, "ws", ws, workspace_of(c, false))) return 0;
     double *b = (double *)ws->data;
     if (x->dtype == GENRE_F32)
@@ -761,7 +766,7 @@ extern "C" int genre_group_norm_backward(const genre_tensor *x, const genre_tens
     const Params p = {weight ? weight->data : nullptr, bias ? bias->data : nullptr, weight ? weight->dtype : 0, bias ? bias->dtype : 0};
     const Map mx = map_of(x), md = map_of(dy);
     const double *s = (const double *)stats->data;
-    const bool small = small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, true);
+    const bool small = small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2);
     if (!check_f64(op, "ws", ws, small ? small_workspace(c.sh) : workspace_of(c, true))) return 0;
     double *b = ws ? (double *)ws->data : nullptr;
     if (small) return small_backward(c.last, x->dtype, c.sh, mx, md, p, g, s, b, st);

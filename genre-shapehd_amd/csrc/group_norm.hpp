@@ -13,14 +13,18 @@ enum { kActNone = 0, kActRelu = 1, kActLeaky = 2, kActSilu = 3 };
 struct F32 { using raw = float; };
 struct F16 { using raw = _Float16; };
 struct BF16 { using raw = __bf16; };
+template <class R, int V> using vec = R __attribute__((ext_vector_type(V), aligned(sizeof(R))));
 
-template <class T, int V>
+// STREAM: past the cache, for maps that do not fit it anyway: a pass's end waits until what it left dirty in the L2s is written
+template <class T, int V, bool STREAM = false>
 __device__ __forceinline__ void store(typename T::raw *p, const float (&v)[V])
 {
-    typename T::raw t[V];
+    typedef vec<typename T::raw, V> W;
+    W t;
 #pragma unroll
     for (int i = 0; i < V; i++) t[i] = (typename T::raw)v[i];              // round to nearest even
-    __builtin_memcpy(p, t, sizeof(t));
+    if (STREAM) __builtin_nontemporal_store(t, (W *)p);
+    else *(W *)p = t;
 }
 
 // Loads and stores of V values need no more than their type's own alignment (gfx950 moves 16 bytes at any address).
@@ -160,8 +164,8 @@ static __global__ __launch_bounds__(256) void channel_grads_kernel(Shape sh, int
 inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 // ---- group_norm_small.hip ---------------------------------------------------------------------------------------
-// whether a call's groups are small enough for it (backward: half as large as forward)
-bool small_fits(bool last, const Shape &sh, int es, bool backward);
+// whether a call's groups are small enough for it
+bool small_fits(bool last, const Shape &sh, int es);
 inline int64_t small_workspace(const Shape &sh) { return sh.N == 1 ? 0 : 2 * (int64_t)sh.N * sh.C; }       // fp64 values, backward
 int small_forward(bool last, int dtype, const Shape &sh, const Map &x, const Map &y, const Params &p, double *stats, hipStream_t st);
 int small_backward(bool last, int dtype, const Shape &sh, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st);

@@ -1,7 +1,6 @@
 // group_norm_small.hip -- group normalisation where one workgroup holds an image's group in its registers.
 //
-// A map whose groups hold up to some 128 (backward: 64) thousand values takes one launch, reads x (and dy) once, and needs no
-// scratch.  A group is `rows` runs of `cols` accesses of V values: channels last, a run is one position's cg channels and every
+// A map whose groups hold up to 16384 values takes one launch, reads x (and dy) once, and needs no scratch.  A group is `rows` runs of `cols` accesses of V values: channels last, a run is one position's cg channels and every
 // thread keeps one column; channels first, a run is one channel's positions, shared by a team of 2^k threads.
 #include "group_norm.hpp"
 
@@ -9,6 +8,8 @@ namespace genre {
 namespace {
 
 using namespace gn;
+
+constexpr int kThreads = 1024, kValues = 16;                               // of the largest workgroup; of a thread
 
 struct Small {
     int rows, cols, team, deep, turns, subs;                               // threads of a run, runs at once, accesses of a thread and run, waves of a team
@@ -74,10 +75,11 @@ struct Walk {
     }
 };
 
-template <class T, int V, int K, bool LAST>
+template <class T, int V, bool LAST>
 __global__ __launch_bounds__(1024) void small_forward_kernel(Map x, Map y, Shape sh, Small m, double *stats, const void *w, const void *b, int wt, int bt)
 {
     using R = typename T::raw;
+    constexpr int K = kValues / V;
     extern __shared__ double coef[];                                       // a and b of the group's channels
     __shared__ double lds[32];
     const int id = by_die(blockIdx.x, gridDim.x), n = id / sh.G, g = id % sh.G;
@@ -128,11 +130,12 @@ __global__ __launch_bounds__(1024) void small_forward_kernel(Map x, Map y, Shape
 }
 
 // chan: the sums of dz and dz (x - mean) by image and channel (more than one image: added up behind this), or dw and db themselves
-template <class T, int V, int K, bool LAST>
-__global__ __launch_bounds__(512) void small_backward_kernel(Map x, Map dy, Map dx, Shape sh, Small m, const double *stats, const void *w, const void *b, int wt,
+template <class T, int V, bool LAST>
+__global__ __launch_bounds__(1024) void small_backward_kernel(Map x, Map dy, Map dx, Shape sh, Small m, const double *stats, const void *w, const void *b, int wt,
                                                              int bt, double2 *chan, void *dw, void *db)
 {
     using R = typename T::raw;
+    constexpr int K = kValues / V;
     extern __shared__ double coef[];                                       // a, b, w; then the sums' scratch
     __shared__ double lds[32];
     const int id = by_die(blockIdx.x, gridDim.x), n = id / sh.G, g = id % sh.G, cg = sh.cg;
@@ -245,11 +248,8 @@ __global__ __launch_bounds__(512) void small_backward_kernel(Map x, Map dy, Map 
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------
-// threads of the largest workgroup, 64 values in each: of x (forward), of x and dy (backward)
-constexpr int kMostForward = 1024, kMostBackward = 512;
-
-// the small form of a call, if its groups fit: values per thread 16 or, in the largest workgroups, 64
-struct SmallCall { Small m; int v, values, threads; };
+// the small form of a call, if its groups fit
+struct SmallCall { Small m; int v, threads; };
 
 int pow2_from(int64_t n)
 {
@@ -258,11 +258,11 @@ int pow2_from(int64_t n)
     return p;
 }
 
-bool small_of(bool last, const Shape &sh, int es, int most, const Map &x, const Map &d, const Map &out, SmallCall &c)
+bool small_of(bool last, const Shape &sh, int es, const Map &x, const Map &d, const Map &out, SmallCall &c)
 {
     const int cg = sh.cg;
     const int64_t S = sh.S;
-    if ((int64_t)cg * S > (int64_t)most * 64 || cg > 1024) return false;
+    if (cg > 1024 || S > kThreads * kValues || cg * S > kThreads * kValues) return false;
     const int64_t run = last ? cg : S;
     c.v = gcd((int)(run & 15), 16 / es);                                   // (run & 15 has run's powers of two up to 8; gcd(0, v) = v)
     if (c.v == 2) c.v = 1;
@@ -275,23 +275,22 @@ bool small_of(bool last, const Shape &sh, int es, int most, const Map &x, const 
     m.gsx = cg * x.sc;
     m.gsd = cg * d.sc;
     m.gso = cg * out.sc;
-    for (c.values = 16; c.values <= 64; c.values *= 4)
-        for (c.threads = c.values == 16 ? 64 : most; c.threads <= most; c.threads *= 2) {
-            const int k = c.values / c.v;
-            m.turns = m.subs = 1;
-            if (last) {
-                m.team = m.cols;
-                m.deep = c.threads / m.team;
-                if (m.deep && (int64_t)m.deep * k >= m.rows) return true;
-                continue;
-            }
-            for (m.team = pow2_from(m.cols) < c.threads ? pow2_from(m.cols) : c.threads; m.team; m.team /= 2) {
-                m.deep = c.threads / m.team;
-                m.turns = (m.cols + m.team - 1) / m.team;
-                m.subs = m.team > 64 ? m.team / 64 : 1;
-                if (m.turns * ((m.rows + m.deep - 1) / m.deep) <= k) return true;
-            }
+    const int k = kValues / c.v;
+    for (c.threads = 64; c.threads <= kThreads; c.threads *= 2) {
+        m.turns = m.subs = 1;
+        if (last) {
+            m.team = m.cols;
+            m.deep = c.threads / m.team;
+            if (m.deep * k >= m.rows) return true;
+            continue;
         }
+        for (m.team = pow2_from(m.cols) < c.threads ? pow2_from(m.cols) : c.threads; m.team; m.team /= 2) {
+            m.deep = c.threads / m.team;
+            m.turns = (m.cols + m.team - 1) / m.team;
+            m.subs = m.team > 64 ? m.team / 64 : 1;
+            if (m.turns * ((m.rows + m.deep - 1) / m.deep) <= k) return true;
+        }
+    }
     return false;
 }
 
@@ -300,21 +299,20 @@ int forward_as(const Shape &sh, const SmallCall &k, const Map &x, const Map &y, 
 {
     const size_t lds = 2 * sizeof(double) * sh.cg;
     const int blocks = sh.N * sh.G;
-    if (k.values == 16) small_forward_kernel<T, V, 16 / V, LAST><<<blocks, k.threads, lds, st>>>(x, y, sh, k.m, stats, p.w, p.b, p.wt, p.bt);
-    else small_forward_kernel<T, V, 64 / V, LAST><<<blocks, k.threads, lds, st>>>(x, y, sh, k.m, stats, p.w, p.b, p.wt, p.bt);
+    small_forward_kernel<T, V, LAST><<<blocks, k.threads, lds, st>>>(x, y, sh, k.m, stats, p.w, p.b, p.wt, p.bt);
     GENRE_LAUNCH_CHECK("group norm");
     return 1;
 }
 
-template <class T, int V, int K, bool LAST>
-int backward_k(const Shape &sh, const SmallCall &k, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
+template <class T, int V, bool LAST>
+int backward_as(const Shape &sh, const SmallCall &k, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
 {
     static std::atomic<uint64_t> reserved{0};
     const bool one = sh.N == 1;
     const size_t lds = sizeof(double) * (3 * sh.cg + (sh.cg & 1)) + sizeof(double2) * (LAST ? V * k.threads : sh.cg * k.m.subs);
-    if (lds > 65536 - 512 && !reserve_lds("group_norm_backward", (const void *)small_backward_kernel<T, V, K, LAST>, 160 * 1024 - 512, reserved)) return 0;
+    if (lds > 65536 - 512 && !reserve_lds("group_norm_backward", (const void *)small_backward_kernel<T, V, LAST>, 160 * 1024 - 512, reserved)) return 0;
     double2 *chan = !one && (g.dw || g.db) ? (double2 *)ws : nullptr;
-    small_backward_kernel<T, V, K, LAST><<<sh.N * sh.G, k.threads, lds, st>>>(x, dy, g.dx, sh, k.m, stats, p.w, p.b, p.wt, p.bt, chan, one ? g.dw : nullptr, one ? g.db : nullptr);
+    small_backward_kernel<T, V, LAST><<<sh.N * sh.G, k.threads, lds, st>>>(x, dy, g.dx, sh, k.m, stats, p.w, p.b, p.wt, p.bt, chan, one ? g.dw : nullptr, one ? g.db : nullptr);
     GENRE_LAUNCH_CHECK("group norm backward");
     if (chan) {
         channel_grads_kernel<<<ceil_div(sh.C, 4), 256, 0, st>>>(sh, 1, chan, stats, g.dw, g.dwt, g.db, g.dbt);
@@ -322,27 +320,21 @@ int backward_k(const Shape &sh, const SmallCall &k, const Map &x, const Map &dy,
     }
     return 1;
 }
-template <class T, int V, bool LAST>
-int backward_as(const Shape &sh, const SmallCall &k, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
-{
-    return k.values == 16 ? backward_k<T, V, 16 / V, LAST>(sh, k, x, dy, p, g, stats, ws, st) : backward_k<T, V, 64 / V, LAST>(sh, k, x, dy, p, g, stats, ws, st);
-}
-
 
 }  // namespace
 
 namespace gn {
 
-bool small_fits(bool last, const Shape &sh, int es, bool backward)
+bool small_fits(bool last, const Shape &sh, int es)
 {
     SmallCall k;
-    return small_of(last, sh, es, backward ? kMostBackward : kMostForward, Map{}, Map{}, Map{}, k);
+    return small_of(last, sh, es, Map{}, Map{}, Map{}, k);
 }
 
 int small_forward(bool last, int dtype, const Shape &sh, const Map &x, const Map &y, const Params &p, double *stats, hipStream_t st)
 {
     SmallCall k;
-    if (!small_of(last, sh, dtype == GENRE_F32 ? 4 : 2, kMostForward, x, x, y, k)) return fail("group norm: the groups are too large for one workgroup");
+    if (!small_of(last, sh, dtype == GENRE_F32 ? 4 : 2, x, x, y, k)) return fail("group norm: the groups are too large for one workgroup");
 #define GENRE_AS(T, V) (last ? forward_as<T, V, true>(sh, k, x, y, p, stats, st) : forward_as<T, V, false>(sh, k, x, y, p, stats, st))
     if (dtype == GENRE_F32) return k.v == 4 ? GENRE_AS(F32, 4) : GENRE_AS(F32, 1);
     if (dtype == GENRE_BF16) return k.v == 8 ? GENRE_AS(BF16, 8) : k.v == 4 ? GENRE_AS(BF16, 4) : GENRE_AS(BF16, 1);
@@ -353,7 +345,7 @@ int small_forward(bool last, int dtype, const Shape &sh, const Map &x, const Map
 int small_backward(bool last, int dtype, const Shape &sh, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
 {
     SmallCall k;
-    if (!small_of(last, sh, dtype == GENRE_F32 ? 4 : 2, kMostBackward, x, dy, g.dx, k)) return fail("group norm: the groups are too large for one workgroup");
+    if (!small_of(last, sh, dtype == GENRE_F32 ? 4 : 2, x, dy, g.dx, k)) return fail("group norm: the groups are too large for one workgroup");
 #define GENRE_AS(T, V) (last ? backward_as<T, V, true>(sh, k, x, dy, p, g, stats, ws, st) : backward_as<T, V, false>(sh, k, x, dy, p, g, stats, ws, st))
     if (dtype == GENRE_F32) return k.v == 4 ? GENRE_AS(F32, 4) : GENRE_AS(F32, 1);
     if (dtype == GENRE_BF16) return k.v == 8 ? GENRE_AS(BF16, 8) : k.v == 4 ? GENRE_AS(BF16, 4) : GENRE_AS(BF16, 1);
