@@ -207,38 +207,37 @@ __global__ __launch_bounds__(512) void last_sums_kernel(Map x, Map dy, Shape sh,
         }
     }
     __syncthreads();
-    // [i][thread] pairs, halved until one period is left; then a channel is its period's values e = channel + m C
-    double2 *pair = (double2 *)lds;
-    const int T0 = blockDim.x;
+    // pairs [i][thread].  A period's `many` values are added up over the periods side by side: `parts` threads each (part by part in
+    // `half`), then a channel's value is the sum of its places e = channel + m C
+    double2 *pair = (double2 *)lds, *half = pair + V * blockDim.x;
+    const int T0 = blockDim.x, places = cut.tile * V, parts = places < T0 ? T0 / places : 1;
 #pragma unroll
     for (int i = 0; i < V; i++) pair[i * T0 + threadIdx.x] = make_double2(s[i], q[i]);
-    for (int live = cut.deep; live > 1;) {
-        const int half = (live + 1) / 2;
-        __syncthreads();
-        if (r + half < live)
-#pragma unroll
-            for (int i = 0; i < V; i++) {
-                const double2 from = pair[i * T0 + threadIdx.x + half * cut.tile];
-                s[i] += from.x;
-                q[i] += from.y;
-                pair[i * T0 + threadIdx.x] = make_double2(s[i], q[i]);
-            }
-        live = half;
-    }
     __syncthreads();
-    const int first = cut.rows == 1 ? at.mid * cut.tile * V : 0, many = cut.rows == 1 ? min(cut.tile * V, sh.C - first) : sh.C;
-    const int64_t row = (int64_t)at.n * cut.chunks + at.chunk;
-    double2 *mine = pair + V * T0;                                         // (with `group`: a tile is all channels)
-    for (int j = threadIdx.x; j < many; j += T0) {
+    for (int j = threadIdx.x; j < parts * places; j += T0) {
+        const int e = j % places;
         double2 t = make_double2(0, 0);
-        for (int m = 0, e = j; m < cut.rows; m++, e += sh.C) {
-            const double2 v = pair[e % V * T0 + e / V];
+        for (int d = j / places; d < cut.deep; d += parts) {
+            const double2 v = pair[e % V * T0 + d * cut.tile + e / V];
             t.x += v.x;
             t.y += v.y;
         }
+        half[j] = t;
+    }
+    __syncthreads();
+    const int first = cut.rows == 1 ? at.mid * places : 0, many = cut.rows == 1 ? min(places, sh.C - first) : sh.C;
+    const int64_t row = (int64_t)at.n * cut.chunks + at.chunk;
+    double2 *mine = pair;                                                  // (with `group`: a tile is all channels)
+    for (int j = threadIdx.x; j < many; j += T0) {
+        double2 t = make_double2(0, 0);
+        for (int m = 0, e = j; m < cut.rows; m++, e += sh.C)
+            for (int d = 0; d < parts; d++) {
+                t.x += half[d * places + e].x;
+                t.y += half[d * places + e].y;
+            }
         if (chan) chan[row * sh.C + first + j] = t;
         if (group) {
-            const double f = OP::kTwo ? load_param(w, wt, j, 1.f) : 1.f;
+            const float f = OP::kTwo ? load_param(w, wt, j, 1.f) : 1.f;
             mine[j] = make_double2(f * t.x, f * t.y);
         }
     }
@@ -467,10 +466,11 @@ inline bool channels_first(const genre_tensor *t) { return t->size[2] == 1 || t-
 inline bool gapless(const genre_tensor *t) { return t->size[2] == 1 || t->stride[2] == t->size[1]; }
 inline Map map_of(const genre_tensor *t) { return {t->data, t->stride[0], t->stride[1], t->size[2] == 1 ? t->size[1] : t->stride[2]}; }
 
-// values per thread and access: 16 bytes; fewer only where a channels-last column may not cross a row's end
+// values per thread and access: 16 bytes; channels last, where each has sums and coefficients of its own, at most four, and fewer
+// where a column may not cross a row's end
 int width_of(const genre_tensor *x, bool last, bool dense)
 {
-    int v = x->dtype == GENRE_F32 ? 4 : 8;
+    int v = last || x->dtype == GENRE_F32 ? 4 : 8;
     if (last) {
         const int C = (int)x->size[1];
         if (!dense || C > 1024 || C / gcd(C, v) > 512) v = gcd(C, v);   // (a period's coefficients and columns have to fit a workgroup)
@@ -529,7 +529,8 @@ struct Call {
     int64_t value_blocks() const { return (int64_t)sh.N * (last ? values.tiles * (int64_t)values.chunks : sh.C * (int64_t)rvalues.chunks); }
     size_t sums_lds(size_t coef) const
     {
-        const size_t a = sizeof(double2) * v * threads + (joined ? sizeof(double2) * sh.C : 0), b = coef_bytes(sh, sums, v, coef);
+        const int places = sums.tile * v, parts = places < threads ? threads / places : 1;
+        const size_t a = sizeof(double2) * (v * threads + parts * places), b = coef_bytes(sh, sums, v, coef);
         return a > b ? a : b;
     }
 };
@@ -608,12 +609,12 @@ Space space_of(const Call &c, bool backward, double *ws)
 template <class T, int V, class OP>
 int sums(const Call &c, const Map &x, const Map &dy, const Params &p, const Between &k, const Space &to, hipStream_t st)
 {
-    if (c.last) {
-        const size_t lds = c.sums_lds(sizeof(typename OP::Coef));
-        last_sums_kernel<T, V, OP><<<(int)c.sums_blocks(), c.threads, lds, st>>>(x, dy, c.sh, c.sums, k, p.w, p.b, p.wt, p.bt, to.chan, to.group);
-    } else if constexpr (V * sizeof(typename T::raw) == 16) {              // (width_of narrows channels-last columns only)
-        first_sums_kernel<T, V, OP><<<(int)c.sums_blocks(), c.threads, 0, st>>>(x, dy, c.sh, c.rsums, k, p.w, p.b, p.wt, p.bt, to.chan);
-    }
+    const int blocks = (int)c.sums_blocks();
+    if constexpr (V <= 4)                                                  // (width_of)
+        if (c.last)
+            last_sums_kernel<T, V, OP><<<blocks, c.threads, c.sums_lds(sizeof(typename OP::Coef)), st>>>(x, dy, c.sh, c.sums, k, p.w, p.b, p.wt, p.bt, to.chan, to.group);
+    if constexpr (V * sizeof(typename T::raw) == 16)
+        if (!c.last) first_sums_kernel<T, V, OP><<<blocks, c.threads, 0, st>>>(x, dy, c.sh, c.rsums, k, p.w, p.b, p.wt, p.bt, to.chan);
     GENRE_LAUNCH_CHECK("group norm sums");
     return 1;
 }
@@ -621,10 +622,11 @@ template <class T, int V, class OP>
 int values(const Call &c, const Map &x, const Map &dy, const Map &out, const Params &p, const Between &k, hipStream_t st)
 {
     const int blocks = (int)k.blocks + (k.dw || k.db ? ceil_div(c.sh.C, c.threads / 64) : 0);
-    if (c.last)
-        last_value_kernel<T, V, OP><<<blocks, c.threads, coef_bytes(c.sh, c.values, V, sizeof(typename OP::Coef)), st>>>(x, dy, out, c.sh, c.values, k, p.w, p.b, p.wt, p.bt);
-    else if constexpr (V * sizeof(typename T::raw) == 16)
-        first_value_kernel<T, V, OP><<<blocks, c.threads, 0, st>>>(x, dy, out, c.sh, c.rvalues, k, p.w, p.b, p.wt, p.bt);
+    if constexpr (V <= 4)
+        if (c.last)
+            last_value_kernel<T, V, OP><<<blocks, c.threads, coef_bytes(c.sh, c.values, V, sizeof(typename OP::Coef)), st>>>(x, dy, out, c.sh, c.values, k, p.w, p.b, p.wt, p.bt);
+    if constexpr (V * sizeof(typename T::raw) == 16)
+        if (!c.last) first_value_kernel<T, V, OP><<<blocks, c.threads, 0, st>>>(x, dy, out, c.sh, c.rvalues, k, p.w, p.b, p.wt, p.bt);
     GENRE_LAUNCH_CHECK("group norm values");
     return 1;
 }
