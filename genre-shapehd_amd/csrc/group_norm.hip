@@ -253,7 +253,7 @@ __global__ __launch_bounds__(512) void last_sums_kernel(Map x, Map dy, Shape sh,
     }
 }
 
-constexpr int kJoinedGroups = 64;
+constexpr int kJoinedGroups = 32;
 
 template <class T, int V, class OP>
 __global__ __launch_bounds__(512) void last_value_kernel(Map x, Map dy, Map out, Shape sh, Cut cut, Between bt, const void *w, const void *b, int wt, int bty)
@@ -540,7 +540,7 @@ void cut_call(Call &c, int64_t N, int64_t C, int64_t S, int groups)
     if (c.last) {
         // the second pass joins the sums where few enough chunks fill half the chip or have few accesses each, and a workgroup sees
         // all channels
-        const int64_t most = kJoined / groups;
+        const int64_t most = kJoined / groups > 64 ? kJoined / groups : 64;
         c.sums = cut_of((int)N, (int)C, S, c.v, kSumsLast, INT32_MAX, &c.threads);
         const int64_t turns = (c.sums.periods + c.sums.deep - 1) / c.sums.deep;
         c.joined = c.sums.tiles == 1 && groups <= kJoinedGroups && C <= 512 && c.threads * c.v <= 2048 &&
@@ -692,7 +692,7 @@ extern "C" int64_t genre_group_norm_workspace(const genre_tensor *x, int groups,
     if (!x) { fail("%s: x is NULL", op); return -1; }
     if (!check_map(op, "x", x, x) || !plan(op, x, nullptr, 0, groups, c)) return -1;
     if (numel(x) == 0) return 0;
-    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2)) return backward ? small_workspace(c.sh) : 0;
+    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, backward != 0)) return backward ? small_workspace(c.sh) : 0;
     int64_t need = workspace_of(c, backward != 0);
     if (c.last) {                                                          // a gap in another map's rows narrows the columns: room for both
         Call d = c;
@@ -725,7 +725,7 @@ extern "C" int genre_group_norm_forward(const genre_tensor *x, const genre_tenso
     const Map mx = map_of(x), my = map_of(y);
     double *s = (double *)stats->data;
     hipStream_t st = (hipStream_t)stream;
-    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2)) return small_forward(c.last, x->dtype, c.sh, mx, my, p, s, st);
+    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, false)) return small_forward(c.last, x->dtype, c.sh, mx, my, p, s, st);
     if (!check_f64(op, "ws", ws, workspace_of(c, false))) return 0;
     double *b = (double *)ws->data;
     if (x->dtype == GENRE_F32)
@@ -768,7 +768,7 @@ extern "C" int genre_group_norm_backward(const genre_tensor *x, const genre_tens
     const Params p = {weight ? weight->data : nullptr, bias ? bias->data : nullptr, weight ? weight->dtype : 0, bias ? bias->dtype : 0};
     const Map mx = map_of(x), md = map_of(dy);
     const double *s = (const double *)stats->data;
-    const bool small = small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2);
+    const bool small = small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, true);
     if (!check_f64(op, "ws", ws, small ? small_workspace(c.sh) : workspace_of(c, true))) return 0;
     double *b = ws ? (double *)ws->data : nullptr;
     if (small) return small_backward(c.last, x->dtype, c.sh, mx, md, p, g, s, b, st);

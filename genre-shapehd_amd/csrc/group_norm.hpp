@@ -2,6 +2,7 @@
 // kernels that walk a map in several passes; group_norm_small.hip: one workgroup per image and group).
 #pragma once
 #include "common.hpp"
+#include "wave_scan.hpp"
 #include <type_traits>
 
 namespace genre {
@@ -102,12 +103,7 @@ struct Shape {
     double m, eps;                                                         // M
 };
 
-__device__ __forceinline__ double wave_sum(double v)
-{
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
+__device__ __forceinline__ double wave_sum(double v) { return wave_last(wave_incl_sum(v)); }
 // sums over the workgroup of two values, in every thread; `lds` has 32 doubles (blockDim.x <= 1024)
 __device__ __forceinline__ void block_sum2(double &a, double &b, double *lds)
 {
@@ -165,7 +161,7 @@ inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 // ---- group_norm_small.hip ---------------------------------------------------------------------------------------
 // whether a call's groups are small enough for it
-bool small_fits(bool last, const Shape &sh, int es);
+bool small_fits(bool last, const Shape &sh, int es, bool backward);
 inline int64_t small_workspace(const Shape &sh) { return sh.N == 1 ? 0 : 2 * (int64_t)sh.N * sh.C; }       // fp64 values, backward
 int small_forward(bool last, int dtype, const Shape &sh, const Map &x, const Map &y, const Params &p, double *stats, hipStream_t st);
 int small_backward(bool last, int dtype, const Shape &sh, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st);

@@ -16,24 +16,28 @@ struct Small {
     int64_t gsx, gsd, gso, psx, psd, pso;                             // a run's stride and a group's in x, dy, out (elements)
 };
 
-// a run-time activation: the launches are short, and a kernel for each would be four times as many
-__device__ __forceinline__ float act_of(int act, double z, float slope)
+// a run-time activation -- a kernel for each would be four times as many -- chosen once around a loop over the values
+template <class F>
+__device__ __forceinline__ void with_act(int act, const F &f)
 {
     switch (act) {
-    case kActRelu: return act_value<kActRelu>(z, slope);
-    case kActLeaky: return act_value<kActLeaky>(z, slope);
-    case kActSilu: return act_value<kActSilu>(z, slope);
-    default: return (float)z;
+    case kActRelu: f(std::integral_constant<int, kActRelu>()); break;
+    case kActLeaky: f(std::integral_constant<int, kActLeaky>()); break;
+    case kActSilu: f(std::integral_constant<int, kActSilu>()); break;
+    default: f(std::integral_constant<int, kActNone>()); break;
     }
 }
-__device__ __forceinline__ float slope_of(int act, double z, float slope)
+
+// sum over each team of 2^k neighbouring lanes (teams of more: over the wave), in every one of them
+__device__ __forceinline__ double team_sum(double v, int team)
 {
-    switch (act) {
-    case kActRelu: return act_slope<kActRelu>(z, slope);
-    case kActLeaky: return act_slope<kActLeaky>(z, slope);
-    case kActSilu: return act_slope<kActSilu>(z, slope);
-    default: return 1.f;
-    }
+    if (team >= 64) return wave_sum(v);
+    if (team >= 2) v += dpp_f64<0xb1, 0xf>(0., v);                         // quad_perm [1,0,3,2]
+    if (team >= 4) v += dpp_f64<0x4e, 0xf>(0., v);                         // quad_perm [2,3,0,1]
+    if (team >= 8) v += dpp_f64<0x141, 0xf>(0., v);                        // row_half_mirror: the other four of eight, equal by now
+    if (team >= 16) v += dpp_f64<0x140, 0xf>(0., v);                       // row_mirror: the other eight
+    if (team >= 32) v += __shfl_xor(v, 16);
+    return v;
 }
 
 // Workgroups go round the eight dies; a die gets consecutive groups here, so that those of one image, whose channels share
@@ -115,18 +119,19 @@ __global__ __launch_bounds__(1024) void small_forward_kernel(Map x, Map y, Shape
         coef[sh.cg + c] = load_param(b, bt, g * sh.cg + c, 0.f);
     }
     __syncthreads();
-    at.restart();
+    with_act(sh.act, [&](auto act) __attribute__((always_inline)) {
+        Walk<LAST> at(m);
 #pragma unroll
-    for (int k = 0; k < K; k++, at.next()) {
-        if (at.here()) {
-            const int c = at.channel(V);
-            float f[V];
-            v[k].fresh();
+        for (int k = 0; k < K; k++, at.next())
+            if (at.here()) {
+                const int c = at.channel(V);
+                float f[V];
+                v[k].fresh();
 #pragma unroll
-            for (int i = 0; i < V; i++) f[i] = act_of(sh.act, fma((double)v[k].at(i) - mean, coef[c + (LAST ? i : 0)], coef[sh.cg + c + (LAST ? i : 0)]), sh.slope);
-            store<T, V>(py + at.row * m.pso + at.col * V, f);
-        }
-    }
+                for (int i = 0; i < V; i++) f[i] = act_value<act>(fma((double)v[k].at(i) - mean, coef[c + (LAST ? i : 0)], coef[sh.cg + c + (LAST ? i : 0)]), sh.slope);
+                store<T, V>(py + at.row * m.pso + at.col * V, f);
+            }
+    });
 }
 
 // chan: the sums of dz and dz (x - mean) by image and channel (more than one image: added up behind this), or dw and db themselves
@@ -162,29 +167,28 @@ __global__ __launch_bounds__(1024) void small_backward_kernel(Map x, Map dy, Map
     double2 acc[LAST ? V : 1];
 #pragma unroll
     for (int i = 0; i < (LAST ? V : 1); i++) acc[i] = make_double2(0, 0);
-    at.restart();
+    with_act(sh.act, [&](auto act) __attribute__((always_inline)) {
+        Walk<LAST> at(m);
 #pragma unroll
-    for (int k = 0; k < K; k++, at.next()) {
-        if (at.here()) {
-            const int c = at.channel(V);
+        for (int k = 0; k < K; k++, at.next()) {
+            if (at.here()) {
+                const int c = at.channel(V);
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                const int e = LAST ? i : 0;
-                const double h = (double)v[k].at(i) - mean, dz = d[k].at(i) * slope_of(sh.act, fma(h, coef[c + e], coef[cg + c + e]), sh.slope);
-                acc[e].x += dz;
-                acc[e].y = fma(dz, h, acc[e].y);
+                for (int i = 0; i < V; i++) {
+                    const int e = LAST ? i : 0;
+                    const double h = (double)v[k].at(i) - mean, dz = d[k].at(i) * act_slope<act>(fma(h, coef[c + e], coef[cg + c + e]), sh.slope);
+                    acc[e].x += dz;
+                    acc[e].y = fma(dz, h, acc[e].y);
+                }
+            }
+            if (!LAST && at.ends_run()) {                                  // (uniform) the run's last turn: its team's sum, wave by wave
+                acc[0].x = team_sum(acc[0].x, m.team);
+                acc[0].y = team_sum(acc[0].y, m.team);
+                if ((int)threadIdx.x % min(m.team, 64) == 0 && at.row < m.rows) scratch[at.row * m.subs + (int)threadIdx.x % m.team / 64] = acc[0];
+                acc[0] = make_double2(0, 0);
             }
         }
-        if (!LAST && at.ends_run()) {                                       // (uniform) the run's last turn: its team's sum, wave by wave
-            const int lanes = m.team < 64 ? m.team : 64;
-            for (int o = lanes / 2; o; o /= 2) {
-                acc[0].x += __shfl_xor(acc[0].x, o);
-                acc[0].y += __shfl_xor(acc[0].y, o);
-            }
-            if ((int)threadIdx.x % lanes == 0 && at.row < m.rows) scratch[at.row * m.subs + (int)threadIdx.x % m.team / 64] = acc[0];
-            acc[0] = make_double2(0, 0);
-        }
-    }
+    });
     if (LAST) {
 #pragma unroll
         for (int i = 0; i < V; i++) scratch[i * blockDim.x + threadIdx.x] = acc[i];
@@ -228,26 +232,28 @@ __global__ __launch_bounds__(1024) void small_backward_kernel(Map x, Map dy, Map
     if (!dx.p) return;                                                     // (uniform)
     block_sum2(m1, m2, lds);
     const double k2 = r * (m1 / sh.m), k3 = r * r * (m2 / sh.m);
-    at.restart();
+    with_act(sh.act, [&](auto act) __attribute__((always_inline)) {
+        Walk<LAST> at(m);
 #pragma unroll
-    for (int k = 0; k < K; k++, at.next()) {
-        if (at.here()) {
-            const int c = at.channel(V);
-            float f[V];
-            v[k].fresh();
-            d[k].fresh();
+        for (int k = 0; k < K; k++, at.next())
+            if (at.here()) {
+                const int c = at.channel(V);
+                float f[V];
+                v[k].fresh();
+                d[k].fresh();
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                const int e = LAST ? i : 0;
-                const double h = (double)v[k].at(i) - mean, dz = d[k].at(i) * slope_of(sh.act, fma(h, coef[c + e], coef[cg + c + e]), sh.slope);
-                f[i] = (float)fma(dz, coef[c + e], -fma(h, k3, k2));
+                for (int i = 0; i < V; i++) {
+                    const int e = LAST ? i : 0;
+                    const double h = (double)v[k].at(i) - mean, dz = d[k].at(i) * act_slope<act>(fma(h, coef[c + e], coef[cg + c + e]), sh.slope);
+                    f[i] = (float)fma(dz, coef[c + e], -fma(h, k3, k2));
+                }
+                store<T, V>(po + at.row * m.pso + at.col * V, f);
             }
-            store<T, V>(po + at.row * m.pso + at.col * V, f);
-        }
-    }
+    });
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------
+constexpr int kBackwardFirst = 4096;
 // the small form of a call, if its groups fit
 struct SmallCall { Small m; int v, threads; };
 
@@ -258,13 +264,15 @@ int pow2_from(int64_t n)
     return p;
 }
 
-bool small_of(bool last, const Shape &sh, int es, const Map &x, const Map &d, const Map &out, SmallCall &c)
+bool small_of(bool last, const Shape &sh, int es, bool backward, const Map &x, const Map &d, const Map &out, SmallCall &c)
 {
     const int cg = sh.cg;
     const int64_t S = sh.S;
-    if (cg > 1024 || S > kThreads * kValues || cg * S > kThreads * kValues) return false;
+    const int most = backward && !last ? kBackwardFirst : kThreads * kValues;
+    if (cg > 1024 || S > most || cg * S > most) return false;
     const int64_t run = last ? cg : S;
-    c.v = gcd((int)(run & 15), 16 / es);                                   // (run & 15 has run's powers of two up to 8; gcd(0, v) = v)
+    // (run & 15 has run's powers of two up to 8; gcd(0, v) = v.)  Channels last, every value of a thread's column has sums of its own
+    c.v = gcd((int)(run & 15), last ? 4 : 16 / es);
     if (c.v == 2) c.v = 1;
     Small &m = c.m;
     m.rows = last ? (int)S : cg;
@@ -325,17 +333,17 @@ int backward_as(const Shape &sh, const SmallCall &k, const Map &x, const Map &dy
 
 namespace gn {
 
-bool small_fits(bool last, const Shape &sh, int es)
+bool small_fits(bool last, const Shape &sh, int es, bool backward)
 {
     SmallCall k;
-    return small_of(last, sh, es, Map{}, Map{}, Map{}, k);
+    return small_of(last, sh, es, backward, Map{}, Map{}, Map{}, k);
 }
 
 int small_forward(bool last, int dtype, const Shape &sh, const Map &x, const Map &y, const Params &p, double *stats, hipStream_t st)
 {
     SmallCall k;
-    if (!small_of(last, sh, dtype == GENRE_F32 ? 4 : 2, x, x, y, k)) return fail("group norm: the groups are too large for one workgroup");
-#define GENRE_AS(T, V) (last ? forward_as<T, V, true>(sh, k, x, y, p, stats, st) : forward_as<T, V, false>(sh, k, x, y, p, stats, st))
+    if (!small_of(last, sh, dtype == GENRE_F32 ? 4 : 2, false, x, x, y, k)) return fail("group norm: the groups are too large for one workgroup");
+#define GENRE_AS(T, V) (last ? forward_as<T, (V) < 4 ? (V) : 4, true>(sh, k, x, y, p, stats, st) : forward_as<T, V, false>(sh, k, x, y, p, stats, st))
     if (dtype == GENRE_F32) return k.v == 4 ? GENRE_AS(F32, 4) : GENRE_AS(F32, 1);
     if (dtype == GENRE_BF16) return k.v == 8 ? GENRE_AS(BF16, 8) : k.v == 4 ? GENRE_AS(BF16, 4) : GENRE_AS(BF16, 1);
     return k.v == 8 ? GENRE_AS(F16, 8) : k.v == 4 ? GENRE_AS(F16, 4) : GENRE_AS(F16, 1);
@@ -345,8 +353,8 @@ int small_forward(bool last, int dtype, const Shape &sh, const Map &x, const Map
 int small_backward(bool last, int dtype, const Shape &sh, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
 {
     SmallCall k;
-    if (!small_of(last, sh, dtype == GENRE_F32 ? 4 : 2, x, dy, g.dx, k)) return fail("group norm: the groups are too large for one workgroup");
-#define GENRE_AS(T, V) (last ? backward_as<T, V, true>(sh, k, x, dy, p, g, stats, ws, st) : backward_as<T, V, false>(sh, k, x, dy, p, g, stats, ws, st))
+    if (!small_of(last, sh, dtype == GENRE_F32 ? 4 : 2, true, x, dy, g.dx, k)) return fail("group norm: the groups are too large for one workgroup");
+#define GENRE_AS(T, V) (last ? backward_as<T, (V) < 4 ? (V) : 4, true>(sh, k, x, dy, p, g, stats, ws, st) : backward_as<T, V, false>(sh, k, x, dy, p, g, stats, ws, st))
     if (dtype == GENRE_F32) return k.v == 4 ? GENRE_AS(F32, 4) : GENRE_AS(F32, 1);
     if (dtype == GENRE_BF16) return k.v == 8 ? GENRE_AS(BF16, 8) : k.v == 4 ? GENRE_AS(BF16, 4) : GENRE_AS(BF16, 1);
     return k.v == 8 ? GENRE_AS(F16, 8) : k.v == 4 ? GENRE_AS(F16, 4) : GENRE_AS(F16, 1);
