@@ -14,6 +14,7 @@ and, for the training step of the networks around them (no counterpart in the re
 
     group_norm_act, GroupNormAct           (toolbox/group_norm)
     grad_norm, clip_grads_, clip_grad_norm_, clip_adam_step_  (toolbox/grad_clip)
+    ClipAdam                               (optim.py)
 
 The directory name carries a hyphen, so import it through the top-level alias
 module ``genre_shapehd_amd`` (repo root), or put this directory (and
@@ -29,9 +30,10 @@ from .toolbox.nndistance.modules.nnd import NNDModule
 from .toolbox.group_norm.functions.group_norm import group_norm_act
 from .toolbox.group_norm.modules.group_norm import GroupNormAct
 from .toolbox.grad_clip.functions.grad_clip import grad_norm, clip_grads_, clip_grad_norm_, clip_adam_step_
+from .optim import ClipAdam
 
 __all__ = ["CameraBackProjection", "SphericalBackProjection", "get_surface_mask",
            "Camera_back_projection_layer", "CalcStopProb", "render_spherical", "sph_pad",
            "gen_sph_grid", "NNDFunction", "nndistance", "nndistance_w_idx", "nndistance_score",
            "NNDModule",
-           "group_norm_act", "GroupNormAct", "grad_norm", "clip_grads_", "clip_grad_norm_", "clip_adam_step_"]
+           "group_norm_act", "GroupNormAct", "grad_norm", "clip_grads_", "clip_grad_norm_", "clip_adam_step_", "ClipAdam"]

@@ -7,7 +7,6 @@
 #include <dlfcn.h>
 
 #include <cmath>
-#include <limits>
 #include <string>
 #include <vector>
 
@@ -354,11 +353,11 @@ Tensor norm_and_factor(const char *op, const Lists &l, int64_t kind, double max_
     return out;
 }
 
-Tensor grad_norm(pybind11::handle tensors, int64_t kind)
+Tensor grad_norm(pybind11::handle tensors, double max_norm, int64_t kind)
 {
     const Lists l = first_list("grad_norm", tensors, false);
     const c10::DeviceGuard guard(l.device);
-    return norm_and_factor("grad_norm", l, kind, std::numeric_limits<double>::infinity()).select(0, 0);
+    return norm_and_factor("grad_norm", l, kind, max_norm);
 }
 
 Tensor clip_grads(pybind11::handle tensors, double max_norm, int64_t kind, bool error_if_nonfinite)
@@ -379,7 +378,7 @@ Tensor clip_grads(pybind11::handle tensors, double max_norm, int64_t kind, bool 
 }
 
 OptTensor adam_step(pybind11::handle params, pybind11::handle grads, pybind11::handle exp_avgs, pybind11::handle exp_avg_sqs, int64_t step, double lr, double beta1,
-                    double beta2, double eps, double weight_decay, bool decoupled, std::optional<double> max_norm, int64_t kind)
+                    double beta2, double eps, double weight_decay, bool decoupled, std::optional<double> max_norm, int64_t kind, const OptTensor &factor)
 {
     const char *op = "clip_adam_step_";
     Lists l = first_list(op, params, true);
@@ -408,8 +407,12 @@ OptTensor adam_step(pybind11::handle params, pybind11::handle grads, pybind11::h
         f = flat(out, GENRE_F32);
         f.data = (float *)f.data + 1;
         f.size[0] = 1;
+    } else if (factor) {
+        TORCH_CHECK(factor->device() == l.device && factor->scalar_type() == at::kFloat && factor->numel() == 1 && factor->layout() == at::kStrided, op,
+                    ": factor must be one fp32 value on ", l.device);
+        f = flat(*factor, GENRE_F32);
     }
-    GENRE_CALL(op, lib.adam_step(l.at[0].data(), l.at[1].data(), l.at[2].data(), l.at[3].data(), l.numel.data(), l.type.data(), l.n(), max_norm ? &f : nullptr,
+    GENRE_CALL(op, lib.adam_step(l.at[0].data(), l.at[1].data(), l.at[2].data(), l.at[3].data(), l.numel.data(), l.type.data(), l.n(), f.data ? &f : nullptr,
                                  step, lr, beta1, beta2, eps, weight_decay, decoupled, st));
     bump(params);
     bump(exp_avgs);

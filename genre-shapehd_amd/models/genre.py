@@ -33,6 +33,7 @@ class GenReOptions:
     net1_path: str = None
     inpaint_path: str = None
     surface_weight: float = 1.0
+    norm: str = "batch"          # of the voxel refiner: "batch" (the reference's) or "group" (networks/networks.py)
 
 
 def Inputs(rgb, silhou, **extra):
@@ -102,7 +103,7 @@ class GenReNet(nn.Module):
         super().__init__()
         opt = opt or GenReOptions()
         self.depth_and_inpaint = DepthInpaintNet(opt)
-        self.refine_net = Unet_3D()
+        self.refine_net = Unet_3D(norm=opt.norm)
         self.proj_depth = Camera_back_projection_layer()
         self.joint_train = opt.joint_train
         self.register_buffer("grid", gen_sph_grid().expand(1, -1, -1, -1, -1).clone())

@@ -6,14 +6,15 @@ import torch
 from torch import nn
 import torch.nn.functional as F
 
+from ..optim import adam
 from ..networks import ImageEncoder, VoxelDecoder, VoxelGenerator, VoxelDiscriminator
 
 
 class MarrNet2Net(nn.Module):
-    def __init__(self, in_planes=4, encode_dims=200, silhou_thres=0, nf=512):
+    def __init__(self, in_planes=4, encode_dims=200, silhou_thres=0, nf=512, norm="batch"):
         super().__init__()
         self.encoder = ImageEncoder(in_planes, encode_dims=encode_dims)
-        self.decoder = VoxelDecoder(n_dims=encode_dims, nf=nf)
+        self.decoder = VoxelDecoder(n_dims=encode_dims, nf=nf, norm=norm)
         self.silhou_thres = silhou_thres
 
     def forward(self, input_struct):
@@ -62,15 +63,16 @@ class WGANGP:
     DistributedDataParallel wrappers: each loss.backward() then all-reduces that network's gradients over RCCL."""
 
     def __init__(self, net_g=None, net_d=None, nz=200, lr=1e-4, betas=(0.5, 0.9), lam=10.0, norm=1.0, d_iter=1,
-                 generator=None):
-        """generator: optional CPU torch.Generator -- latent codes and the interpolation weights of the penalty are then
+                 generator=None, gen_norm="batch", clip_grad=None):
+        """gen_norm: the default generator's normalisation, "batch" or "group".  clip_grad: bound on the norm of each network's
+        gradients (ClipAdam; None: not bounded, as in the reference).  generator: optional CPU torch.Generator -- latent codes and the interpolation weights of the penalty are then
         drawn on the host from it and copied to the device (a run is reproducible across devices); default: drawn on
         the device, as the reference does (wgangp.py:98,134)"""
-        self.net_g = net_g if net_g is not None else VoxelGenerator(nz)
+        self.net_g = net_g if net_g is not None else VoxelGenerator(nz, norm=gen_norm)
         self.net_d = net_d if net_d is not None else VoxelDiscriminator()
         self.nz, self.lam, self.norm, self.d_iter = nz, lam, norm, d_iter
-        self.opt_g = torch.optim.Adam(self.net_g.parameters(), lr=lr, betas=betas)
-        self.opt_d = torch.optim.Adam(self.net_d.parameters(), lr=lr, betas=betas)
+        self.opt_g = adam(self.net_g.parameters(), lr, betas, clip_grad)
+        self.opt_d = adam(self.net_d.parameters(), lr, betas, clip_grad)
         self._last_err_g = None
         self.generator = generator
 

@@ -7,9 +7,17 @@
   VoxelDiscriminator  3-D WGAN-GP critic                                               (:111-144)
 
 Layer lists are written as tables; `nn.Sequential` indices and attribute names equal the reference's so that its
-state_dicts load (including the two empty placeholders inside VoxelDecoder.main that keep old checkpoints aligned)."""
+state_dicts load (including the two empty placeholders inside VoxelDecoder.main that keep old checkpoints aligned).
+
+norm="group" (Unet_3D, VoxelDecoder, VoxelGenerator; GPU only) puts GroupNormAct in the place of BatchNorm and its activation:
+statistics of one image, whatever the batch and the number of ranks, and training on a batch of one.  The convolutions keep
+their names, so that their weights load from a checkpoint with strict=False."""
+import math
+
 import torch
 from torch import nn
+
+from ..toolbox.group_norm.modules.group_norm import GroupNormAct
 
 from .resnet import resnet18
 from .thin_conv import ThinConv3d, ThinConvTranspose3d
@@ -29,8 +37,18 @@ def _down3(cin, cout, bias):               # /2
     return ThinConv3d(cin, cout, 4, 2, 1, bias=bias)
 
 
-def _bn_relu3(c):
-    return [nn.BatchNorm3d(c), nn.ReLU(inplace=True)]
+def _norm_act3(c, norm, act):
+    """[normalisation, activation] of c channels; "group": one operator does both, and an empty module keeps the indices"""
+    if norm == "group":
+        name, slope = ("relu", 0.0) if isinstance(act, nn.ReLU) else ("leaky_relu", act.negative_slope)
+        return [GroupNormAct(math.gcd(c, 8), c, act=name, slope=slope), nn.Identity()]
+    if norm != "batch":
+        raise ValueError("norm must be 'batch' or 'group', got %r" % (norm,))
+    return [nn.BatchNorm3d(c), act]
+
+
+def _norm_relu3(c, norm):
+    return _norm_act3(c, norm, nn.ReLU(inplace=True))
 
 
 class ViewAsLinear(nn.Module):
@@ -53,14 +71,14 @@ class ImageEncoder(nn.Module):
 
 
 class VoxelDecoder(nn.Module):
-    def __init__(self, n_dims=200, nf=512):
+    def __init__(self, n_dims=200, nf=512, norm="batch"):
         super().__init__()
-        layers = [_grow3(n_dims, nf, True), *_bn_relu3(nf),
-                  _up3(nf, nf // 2, True), *_bn_relu3(nf // 2),
+        layers = [_grow3(n_dims, nf, True), *_norm_relu3(nf, norm),
+                  _up3(nf, nf // 2, True), *_norm_relu3(nf // 2, norm),
                   nn.Sequential(), nn.Sequential()]               # placeholders: indices of released checkpoints
         c = nf // 2
         for _ in range(3):
-            layers += [_up3(c, c // 2, True), *_bn_relu3(c // 2)]
+            layers += [_up3(c, c // 2, True), *_norm_relu3(c // 2, norm)]
             c //= 2
         layers.append(_up3(c, 1, True))
         self.main = nn.Sequential(*layers)
@@ -70,15 +88,15 @@ class VoxelDecoder(nn.Module):
 
 
 class VoxelGenerator(nn.Module):
-    def __init__(self, nz=200, nf=64, bias=False, res=128):
+    def __init__(self, nz=200, nf=64, bias=False, res=128, norm="batch"):
         super().__init__()
         if res not in (64, 128):
             raise NotImplementedError(res)
-        layers = [_grow3(nz, nf * 8, bias), *_bn_relu3(nf * 8)]
+        layers = [_grow3(nz, nf * 8, bias), *_norm_relu3(nf * 8, norm)]
         for cin, cout in ((8, 4), (4, 2), (2, 1)):                # 4^3 -> 32^3
-            layers += [_up3(nf * cin, nf * cout, bias), *_bn_relu3(nf * cout)]
+            layers += [_up3(nf * cin, nf * cout, bias), *_norm_relu3(nf * cout, norm)]
         if res == 128:
-            layers += [_up3(nf, nf, bias), *_bn_relu3(nf)]        # -> 64^3
+            layers += [_up3(nf, nf, bias), *_norm_relu3(nf, norm)]        # -> 64^3
         layers += [_up3(nf, 1, bias), nn.Sigmoid()]
         self.main = nn.Sequential(*layers)
 
@@ -103,19 +121,19 @@ class VoxelDiscriminator(nn.Module):
 
 
 class Conv3d_block(nn.Module):
-    def __init__(self, ncin, ncout, kernel_size, stride, pad, dropout=False):
+    def __init__(self, ncin, ncout, kernel_size, stride, pad, dropout=False, norm="batch"):
         super().__init__()
-        self.net = nn.Sequential(ThinConv3d(ncin, ncout, kernel_size, stride, pad), nn.BatchNorm3d(ncout), nn.LeakyReLU())
+        self.net = nn.Sequential(ThinConv3d(ncin, ncout, kernel_size, stride, pad), *_norm_act3(ncout, norm, nn.LeakyReLU()))
 
     def forward(self, x):
         return self.net(x)
 
 
 class Deconv3d_skip(nn.Module):
-    def __init__(self, ncin, ncout, kernel_size, stride, pad, extra=0, is_activate=True):
+    def __init__(self, ncin, ncout, kernel_size, stride, pad, extra=0, is_activate=True, norm="batch"):
         super().__init__()
         up = ThinConvTranspose3d(ncin, ncout, kernel_size, stride, pad, extra)
-        self.net = nn.Sequential(up, nn.BatchNorm3d(ncout), nn.LeakyReLU()) if is_activate else up
+        self.net = nn.Sequential(up, *_norm_act3(ncout, norm, nn.LeakyReLU())) if is_activate else up
 
     def forward(self, x, skip_in):
         return self.net(torch.cat((x, skip_in), 1))
@@ -127,18 +145,18 @@ class Unet_3D(nn.Module):
     ENC = ((8, 2, 3), (4, 2, 1), (4, 2, 1), (4, 2, 1), (4, 2, 1), (4, 1, 0))
     DEC = ((4, 1, 0), (4, 2, 1), (4, 2, 1), (4, 2, 1), (8, 2, 3), (4, 2, 1))
 
-    def __init__(self, nf=20, in_channel=2, no_linear=False):
+    def __init__(self, nf=20, in_channel=2, no_linear=False, norm="batch"):
         super().__init__()
         self.nf = nf
         self.no_linear = no_linear
         w = [in_channel] + [nf << i for i in range(6)]            # 2, nf, 2nf, ... 32nf
         for i, (k, s, p) in enumerate(self.ENC):
-            setattr(self, "enc%d" % (i + 1), Conv3d_block(w[i], w[i + 1], k, s, p))
+            setattr(self, "enc%d" % (i + 1), Conv3d_block(w[i], w[i + 1], k, s, p, norm=norm))
         self.full_conv_block = nn.Sequential(nn.Linear(32 * nf, 32 * nf), nn.LeakyReLU())
         for i in range(6):                                          # dec(i+1) undoes enc(6-i); input = previous + skip
             k, s, p = self.DEC[i]
             cout = w[5 - i] if i < 5 else 1
-            setattr(self, "dec%d" % (i + 1), Deconv3d_skip(2 * w[6 - i], cout, k, s, p, 0, is_activate=i < 5))
+            setattr(self, "dec%d" % (i + 1), Deconv3d_skip(2 * w[6 - i], cout, k, s, p, 0, is_activate=i < 5, norm=norm))
 
     def forward(self, x):
         enc = []

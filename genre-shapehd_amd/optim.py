@@ -1,0 +1,73 @@
+"""The optimiser of the training commands with a bound on the gradients: Adam whose step takes the global clip with it."""
+import torch
+
+from .toolbox.grad_clip.functions.grad_clip import _native, clip_adam_step_
+
+
+class ClipAdam(torch.optim.Adam):
+    """torch.optim.Adam (state_dicts go from one to the other) on GPU tensors, as if
+    torch.nn.utils.clip_grad_norm_(all parameters, max_grad_norm) had run before every step, in a few launches for the whole
+    network: the gradients are read twice and never written.  The norm that a step found is left in `grad_norm`, on the GPU.
+
+    The moments are fp32 whatever the weights' type.  Parameters without a gradient are passed over, as they are there."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0, max_grad_norm=None, decoupled_weight_decay=False):
+        if max_grad_norm is not None and not max_grad_norm >= 0:
+            raise ValueError("max_grad_norm must not be negative, got %r" % (max_grad_norm,))
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, decoupled_weight_decay=decoupled_weight_decay)
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm = None
+
+    def _moments(self, p):
+        st = self.state[p]
+        if not st:
+            st["step"] = torch.tensor(0.0)
+            st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+            st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+        elif st["exp_avg"].dtype != torch.float32:                     # a loaded state takes the weights' type
+            st["exp_avg"], st["exp_avg_sq"] = st["exp_avg"].float(), st["exp_avg_sq"].float()
+        return st
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        # what is stepped together: the same options and the same number of steps behind it (`step` tensors are shared by those)
+        batches, every = [], []
+        for group in self.param_groups:
+            if any(group.get(k) for k in ("amsgrad", "maximize", "capturable", "differentiable")):
+                raise RuntimeError("ClipAdam: amsgrad, maximize, capturable and differentiable are not supported")
+            counts, found = {}, {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                st = self._moments(p)
+                key = id(st["step"])
+                if key not in counts:
+                    counts[key] = int(st["step"])
+                found.setdefault(counts[key], []).append((p, p.grad, st))
+                every.append(p.grad)
+            batches += [(group, count, members) for count, members in found.items()]
+        if not every:
+            return loss
+        factor = None
+        if self.max_grad_norm is not None:
+            self.grad_norm, factor = _native.grad_norm(every, float(self.max_grad_norm), 2)
+        for group, count, members in batches:
+            params, grads, states = zip(*members)
+            clip_adam_step_(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], count + 1, lr=float(group["lr"]),
+                            betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                            decoupled=group.get("decoupled_weight_decay", False), factor=factor)
+            now = torch.tensor(float(count + 1))
+            for s in states:
+                s["step"] = now
+        return loss
+
+
+def adam(params, lr, betas, clip_grad=None):
+    """the optimiser of the training commands: torch.optim.Adam, or with a bound on the gradients' norm ClipAdam"""
+    if clip_grad is None:
+        return torch.optim.Adam(params, lr=lr, betas=betas)
+    return ClipAdam(params, lr=lr, betas=betas, max_grad_norm=clip_grad)

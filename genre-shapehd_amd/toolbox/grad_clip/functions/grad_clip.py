@@ -33,7 +33,7 @@ def grad_norm(tensors, norm_type=2.0):
     """norm of the vector of all the tensors' values (2: Euclidean, fp64 sums; inf: the largest magnitude) as an fp32 tensor of no
     dimensions on their GPU.  NaN where a value is NaN.  An empty list has the norm 0 (on the CPU, as nothing names a GPU)."""
     kind, tensors = _kind("grad_norm", norm_type), _list(tensors)
-    return _native.grad_norm(tensors, kind) if tensors else torch.tensor(0.0)
+    return _native.grad_norm(tensors, math.inf, kind)[0] if tensors else torch.tensor(0.0)
 
 
 def clip_grads_(tensors, max_norm, norm_type=2.0, error_if_nonfinite=False):
@@ -51,12 +51,16 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
 
 
 def clip_adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled=False,
-                    max_norm=None, norm_type=2.0):
+                    max_norm=None, norm_type=2.0, factor=None):
     """one Adam step on `params` in place, `exp_avgs` and `exp_avg_sqs` with them, as if clip_grads_(grads, max_norm, norm_type) had
     run before -- without writing the gradients.  step counts from 1.  weight_decay is added to the gradient, or (decoupled) shrinks
     the weights by lr * weight_decay.  params[i] and grads[i] have one type and layout, the states are fp32 in that layout; no two
-    tensors may overlap.  Returns the norm of the gradients before the clip (None without max_norm)."""
+    tensors may overlap.  Returns the norm of the gradients before the clip (None without max_norm).
+    factor (instead of max_norm): one fp32 value on the same GPU that the gradients are multiplied by -- for weights that are
+    stepped in several calls under one clip."""
     kind = _kind("clip_adam_step_", norm_type)
+    if factor is not None and max_norm is not None:
+        raise RuntimeError("clip_adam_step_: max_norm or factor, not both")
     params, grads, exp_avgs, exp_avg_sqs = lists = [_list(ts) for ts in (params, grads, exp_avgs, exp_avg_sqs)]
     if any(len(ts) != len(params) for ts in lists):
         raise RuntimeError("clip_adam_step_: the four lists have %s tensors" % [len(ts) for ts in lists])
@@ -68,4 +72,4 @@ def clip_adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, beta
                            % ((betas, lr, eps, weight_decay, step),))
     if not params:
         return None if max_norm is None else torch.tensor(0.0)
-    return _native.adam_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, decoupled, max_norm, kind)
+    return _native.adam_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps, weight_decay, decoupled, max_norm, kind, factor)

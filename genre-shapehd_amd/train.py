@@ -29,6 +29,7 @@ except ImportError:                                   # run as a script from any
     import genre_shapehd_amd                          # noqa: F401
 from genre_shapehd_amd import dist_utils              # noqa: E402
 from genre_shapehd_amd.models import shapehd as M_shapehd, checkpoint     # noqa: E402
+from genre_shapehd_amd.optim import adam                                  # noqa: E402
 
 
 # ---- synthetic batches (shapes of datasets/shapenet.py after preprocessing) ---------------------------------
@@ -138,6 +139,9 @@ def main(argv=None):
     ap.add_argument("--lr", type=float, default=1e-4)
     ap.add_argument("--w_gan_loss", type=float, default=1e-3)
     ap.add_argument("--chamfer_weight", type=float, default=0.0)
+    ap.add_argument("--clip_grad", type=float, default=None, help="bound on the norm of a network's gradients together (default: none)")
+    ap.add_argument("--norm", choices=["batch", "group"], default="batch",
+                    help="normalisation of the trained 3-D network (shapehd: voxel decoder, wgangp: generator, genre: refiner)")
     ap.add_argument("--backend", default=None)
     ap.add_argument("--save", default=None)
     ap.add_argument("--resume", default=None)
@@ -155,22 +159,22 @@ def main(argv=None):
     torch.manual_seed(1234)                                             # identical initial weights on every rank
     start = 0
     if args.config == "shapehd":
-        net = M_shapehd.ShapeHDNet().to(device)
+        net = M_shapehd.ShapeHDNet(norm=args.norm).to(device)
         model = ddp(net, device, dist)
-        optim = torch.optim.Adam(net.marrnet2.parameters(), lr=args.lr, betas=(0.5, 0.9))
+        optim = adam(net.marrnet2.parameters(), args.lr, (0.5, 0.9), args.clip_grad)
         nets, optims = [net], [optim]
     elif args.config == "wgangp":
-        gan = M_shapehd.WGANGP(lr=args.lr)
+        gan = M_shapehd.WGANGP(lr=args.lr, gen_norm=args.norm, clip_grad=args.clip_grad)
         gan.net_g.to(device), gan.net_d.to(device)
         raw_g, raw_d = gan.net_g, gan.net_d
         gan.net_g, gan.net_d = ddp(raw_g, device, dist), ddp(raw_d, device, dist)
         nets, optims = [raw_g, raw_d], [gan.opt_g, gan.opt_d]
     else:
         from genre_shapehd_amd.models.genre import GenReNet, GenReOptions
-        gopt = GenReOptions(joint_train=True)
+        gopt = GenReOptions(joint_train=True, norm=args.norm)
         net = GenReNet(gopt).to(device)
         model = ddp(net, device, dist)
-        optim = torch.optim.Adam(net.parameters(), lr=args.lr, betas=(0.5, 0.9))
+        optim = adam(net.parameters(), args.lr, (0.5, 0.9), args.clip_grad)
         nets, optims = [net], [optim]
     if args.resume:
         extra = checkpoint.load_state_dict(args.resume, nets, optims)

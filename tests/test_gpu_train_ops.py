@@ -1,0 +1,216 @@
+"""Group norm, clip and Adam as the training step uses them together: networks with norm="group", ClipAdam, the training command.
+Bounds are those of test_gpu_group_norm.py and test_gpu_grad_clip.py, held by every operator on what it was really given."""
+import pytest
+import torch
+
+from test_gpu_grad_clip import U, adam64, factor64, norm64
+from test_gpu_group_norm import LAST, definition, near
+
+pytestmark = pytest.mark.gpu
+
+
+def networks(genre):
+    from genre_shapehd_amd import networks
+    return networks
+
+
+def watch(net, genre):
+    """{module: what its group norm read, gave and received} of the next forward and backward"""
+    seen, hooks = {}, []
+
+    def forward(m, args, y):
+        x, s = args[0], seen.setdefault(m, {})
+        s["x"], s["y"] = x.detach().clone(), y.detach().clone()
+        x.register_hook(lambda g, s=s: s.__setitem__("dx", g.detach().clone()))
+        y.register_hook(lambda g, s=s: s.__setitem__("dy", g.detach().clone()))
+
+    for m in net.modules():
+        if isinstance(m, genre.GroupNormAct):
+            hooks.append(m.register_forward_hook(forward))
+    return seen, hooks
+
+
+@pytest.mark.parametrize("layout", ("first", "last"))
+@pytest.mark.parametrize("kind", ("decoder", "generator"))
+def test_a_training_step_of_a_decoder(genre, dev, kind, layout):
+    torch.manual_seed(0)
+    N = networks(genre)
+    net = (N.VoxelDecoder(n_dims=12, nf=32, norm="group") if kind == "decoder" else N.VoxelGenerator(nz=12, nf=4, res=64, norm="group")).to(dev)
+    if layout == "last":
+        net = net.to(memory_format=LAST[5])
+    opt = genre.ClipAdam(net.parameters(), lr=1e-3, betas=(0.5, 0.9), max_grad_norm=1e-3)
+    for step in (1, 2):
+        seen, hooks = watch(net, genre)
+        code = torch.randn(2, 12, 1, 1, 1, device=dev)
+        opt.zero_grad(set_to_none=True)
+        out = net(code)
+        torch.nn.functional.mse_loss(out, torch.rand_like(out)).backward()
+        for h in hooks:
+            h.remove()
+        assert len(seen) == (5 if kind == "decoder" else 4)
+        for m, s in seen.items():
+            want = definition(s["x"], s["dy"], m.weight, m.bias, m.num_groups, m.act, m.eps, m.slope)
+            for got, k in ((s["y"], "y"), (s["dx"], "dx"), (m.weight.grad, "dw"), (m.bias.grad, "db")):
+                near(got, want[k], "%s of %s" % (k, tuple(s["x"].shape)))
+        ps = list(net.parameters())
+        grads, before = [p.grad.clone() for p in ps], [p.detach().clone() for p in ps]
+        states = [(opt.state[p].get("exp_avg", torch.zeros_like(p)).clone(), opt.state[p].get("exp_avg_sq", torch.zeros_like(p)).clone()) for p in ps]
+        opt.step()
+        norm = norm64(grads)
+        f = factor64(norm, 1e-3)
+        assert abs(opt.grad_norm.item() - norm) <= 1.1 * U * norm and f < 1
+        for p, b, g, (m, v) in zip(ps, before, grads, states):
+            assert torch.equal(p.grad, g)
+            for got, (value, bound) in zip((p, opt.state[p]["exp_avg"], opt.state[p]["exp_avg_sq"]), adam64(b, g, m, v, step, 1e-3, (0.5, 0.9), 1e-8, 0.0, False, f, p.dtype)):
+                assert bool(((got.detach().double().cpu() - value).abs() <= bound + 1e-38).all())
+            assert float(opt.state[p]["step"]) == step
+
+
+def test_the_refiner_trains_on_one_image(genre, dev):
+    """its innermost map is 1^3: batch statistics of one image do not exist, group statistics do"""
+    N = networks(genre)
+    x = torch.rand(1, 2, 128, 128, 128, device=dev)
+    with pytest.raises(ValueError):
+        N.Unet_3D(nf=2).to(dev)(x)
+    net = N.Unet_3D(nf=2, norm="group").to(dev)
+    seen, hooks = watch(net, genre)
+    net(x).square().mean().backward()
+    assert len(seen) == 11
+    for m, s in seen.items():
+        want = definition(s["x"], s["dy"], m.weight, m.bias, m.num_groups, m.act, m.eps, m.slope)
+        near(s["y"], want["y"], "y")
+        near(s["dx"], want["dx"], "dx")
+    assert all(p.grad is not None and bool(p.grad.isfinite().all()) for p in net.parameters())
+
+
+def test_an_image_does_not_depend_on_its_batch(genre, dev):
+    x, w, b = torch.randn(4, 40, 9, 10, 11, device=dev), torch.randn(40, device=dev), torch.randn(40, device=dev)
+    for last in (False, True):
+        x = x.contiguous(memory_format=LAST[5] if last else torch.contiguous_format)
+        whole = genre.group_norm_act(x, 8, w, b, act="silu")
+        for i in range(4):
+            near(genre.group_norm_act(x[i:i + 1], 8, w, b, act="silu"),
+                 definition(x[i:i + 1], torch.zeros_like(x[i:i + 1]), w, b, 8, "silu", 1e-5, 0.01)["y"], "alone")
+            near(whole[i:i + 1], definition(x[i:i + 1], torch.zeros_like(x[i:i + 1]), w, b, 8, "silu", 1e-5, 0.01)["y"], "in the batch")
+
+
+# ---- ClipAdam ---------------------------------------------------------------------------------------------------
+def weights(dev, seed=0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.nn.Parameter((0.1 * torch.randn(s, generator=g)).to(dtype).to(dev)) for s in ((20, 7, 3, 3), (20,), (1,), (33, 65))]
+
+
+def test_steps_with_parameters_that_come_and_go(genre, dev):
+    """a parameter without a gradient keeps its moments and its count; the others go on: torch.optim.Adam in float64 says where to.
+    Bound: each of 4 steps adds that of test_gpu_grad_clip's five, 20 u lr 4 + 2 u |p|"""
+    ps = weights(dev)
+    ref = [p.detach().double().requires_grad_(True) for p in ps]
+    opt = genre.ClipAdam([{"params": ps[:2]}, {"params": ps[2:], "lr": 5e-3, "weight_decay": 0.01}], lr=1e-2, betas=(0.5, 0.9), max_grad_norm=2.0)
+    stock = torch.optim.Adam([{"params": ref[:2]}, {"params": ref[2:], "lr": 5e-3, "weight_decay": 0.01}], lr=1e-2, betas=(0.5, 0.9))
+    for step in range(4):
+        g = torch.Generator().manual_seed(100 + step)
+        for i, (p, r) in enumerate(zip(ps, ref)):
+            p.grad = None if (step + i) % 3 == 0 else torch.randn(p.shape, generator=g).to(dev)
+            r.grad = None if p.grad is None else p.grad.double()
+        torch.nn.utils.clip_grad_norm_(ref, 2.0)
+        stock.step()
+        opt.step()
+    for p, r in zip(ps, ref):
+        assert float(opt.state[p]["step"]) == float(stock.state[r]["step"])
+        assert bool(((p.double() - r).abs() <= 4 * (20 * U * 1e-2 * 4 + 2 * U * r.abs())).all())
+
+
+def test_states_go_to_torch_and_back(genre, dev, tmp_path):
+    from genre_shapehd_amd.models import checkpoint
+    for dtype in (torch.float32, torch.bfloat16):
+        ps = weights(dev, 1, dtype)
+        opt = genre.ClipAdam(ps, lr=1e-2, betas=(0.5, 0.9), max_grad_norm=1.0)
+        for p in ps:
+            p.grad = torch.randn_like(p)
+        opt.step()
+        net = torch.nn.Module()
+        net.ps = torch.nn.ParameterList(ps)
+        path = str(tmp_path / "c.pt")
+        checkpoint.save_state_dict(path, [net], [opt], epoch=3)
+        others = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+        again = genre.ClipAdam(others, lr=1e-2, betas=(0.5, 0.9), max_grad_norm=1.0)
+        stock = torch.optim.Adam([torch.nn.Parameter(p.detach().clone()) for p in ps], lr=1e-2, betas=(0.5, 0.9))
+        net2 = torch.nn.Module()
+        net2.ps = torch.nn.ParameterList(others)
+        assert checkpoint.load_state_dict(path, [net2], [again])["epoch"] == 3
+        stock.load_state_dict(opt.state_dict())
+        for p, o, s in zip(ps, others, stock.param_groups[0]["params"]):
+            assert float(stock.state[s]["step"]) == float(again.state[o]["step"]) == 1
+            o.grad = p.grad.clone()
+        if dtype == torch.float32:                                        # (torch keeps bf16 moments: rounded on the way)
+            opt.step()
+            again.step()
+            assert all(torch.equal(p, o) for p, o in zip(ps, others))
+        # a state that torch's Adam wrote
+        third = genre.ClipAdam([torch.nn.Parameter(p.detach().clone()) for p in ps], lr=1e-2, betas=(0.5, 0.9))
+        third.load_state_dict(stock.state_dict())
+        for p, q in zip(third.param_groups[0]["params"], ps):
+            p.grad = torch.ones_like(p)
+        third.step()
+        assert all(st["exp_avg"].dtype == torch.float32 and float(st["step"]) == 2 for st in third.state.values())
+
+
+def test_a_step_without_a_bound_and_one_without_gradients(genre, dev):
+    ps = weights(dev, 2)
+    opt = genre.ClipAdam(ps, lr=1e-2)
+    before = [p.detach().clone() for p in ps]
+    assert opt.step(lambda: 3.0) == 3.0
+    assert all(torch.equal(p, b) for p, b in zip(ps, before)) and opt.grad_norm is None
+    for p in ps:
+        p.grad = 5 * torch.ones_like(p)
+    opt.step()
+    assert opt.grad_norm is None
+    # a first step of constant gradients: m / sqrt(v) = 1, so p falls by lr (g / (g + eps)): 12 u lr + 2 u |p|
+    assert all(bool(((p - (b - 1e-2)).abs() <= 12 * U * 1e-2 + 3 * U * b.abs() + 1e-10).all()) for p, b in zip(ps, before))
+
+
+def test_weights_that_a_graph_still_needs_are_seen_to_change(genre, dev):
+    """in-place steps count as such: a backward through what a step has overwritten raises, as after torch's optimisers"""
+    p = torch.nn.Parameter(torch.randn(5, device=dev))
+    loss = (p * p).sum()
+    p.grad = torch.ones_like(p)
+    genre.ClipAdam([p]).step()
+    with pytest.raises(RuntimeError):
+        loss.backward()
+
+
+@pytest.mark.parametrize("config", ("shapehd", "wgangp", "genre"))
+def test_the_training_command(genre, dev, config, monkeypatch, capsys, tmp_path):
+    """two steps of train.py with both options, on narrow networks (and without MIOpen's search, which takes minutes for new shapes)"""
+    from functools import partial
+    from genre_shapehd_amd import networks, train
+    from genre_shapehd_amd.models import genre as M_genre, shapehd as M_shapehd
+    made = []
+
+    def watched(*args):
+        made.append(optim(*args))
+        return made[-1]
+
+    optim = train.adam
+
+    class Quiet:                                                          # (what is set on it does not reach torch)
+        def __getattr__(self, name, real=torch.backends.cudnn):
+            return getattr(real, name)
+
+    monkeypatch.setattr(torch.backends, "cudnn", Quiet())
+    monkeypatch.setattr(train, "adam", watched)
+    monkeypatch.setattr(M_shapehd, "adam", watched)
+    monkeypatch.setattr(M_shapehd, "ShapeHDNet", partial(M_shapehd.ShapeHDNet, nf=32, d_nf=2))
+    monkeypatch.setattr(M_shapehd, "VoxelGenerator", partial(networks.VoxelGenerator, nf=2))
+    monkeypatch.setattr(M_shapehd, "VoxelDiscriminator", partial(networks.VoxelDiscriminator, nf=2))
+    monkeypatch.setattr(M_genre, "Unet_3D", partial(networks.Unet_3D, nf=2))
+    path = str(tmp_path / "c.pt")
+    args = ["--config", config, "--norm", "group", "--clip_grad", "0.5", "--batch", "2", "--steps", "2", "--save", path]
+    train.main(args)
+    train.main(args + ["--resume", path])
+    lines = [line.split() for line in capsys.readouterr().out.splitlines() if line.startswith("step")]
+    assert [line[1] for line in lines] == ["0", "1", "2", "3"]
+    nets = 2 if config == "wgangp" else 1
+    assert len(made) == 2 * nets and all(type(o) is genre.ClipAdam and float(o.grad_norm) > 0 for o in made)
+    for first, again in zip(made[:nets], made[nets:]):
+        assert {float(s["step"]) for s in first.state.values()} == {2.0} and {float(s["step"]) for s in again.state.values()} == {4.0}
