@@ -72,12 +72,20 @@ __device__ __forceinline__ double2 group_total(const Shape &sh, int chunks, cons
 {
     const double2 *p = chan + (int64_t)n * chunks * sh.C + g * sh.cg;
     double2 t = make_double2(0, 0);
-    for (unsigned i = threadIdx.x; i < (unsigned)chunks * sh.cg; i += blockDim.x) {
-        const unsigned row = i / (unsigned)sh.cg, c = i % (unsigned)sh.cg;
+    const unsigned cg = sh.cg, rows = blockDim.x / cg, rest = blockDim.x % cg;
+    unsigned row = threadIdx.x / cg, c = threadIdx.x % cg;
+#pragma unroll 4
+    while (row < (unsigned)chunks) {
         const double2 v = p[(int64_t)row * sh.C + c];
-        const double f = TWO ? load_param(w, wt, g * sh.cg + c, 1.f) : 1.f;
+        const float f = TWO ? load_param(w, wt, g * sh.cg + c, 1.f) : 1.f;
         t.x = fma(f, v.x, t.x);
         t.y = fma(f, v.y, t.y);
+        row += rows;
+        c += rest;
+        if (c >= cg) {
+            c -= cg;
+            row++;
+        }
     }
     block_sum2(t.x, t.y, lds);
     return t;
@@ -158,8 +166,11 @@ inline size_t coef_bytes(const Shape &sh, const Cut &cut, int v, size_t coef)
     return coef * (cut.rows == 1 ? (cut.tile * v < sh.C ? cut.tile * v : sh.C) : sh.C);
 }
 
+// columns (and threads) of a workgroup: where a column is a single value, rows of up to 1024 stay in one
+constexpr int columns_of(int v) { return v == 1 ? 1024 : 512; }
+
 template <class T, int V, class OP>
-__global__ __launch_bounds__(512) void last_sums_kernel(Map x, Map dy, Shape sh, Cut cut, Between bt, const void *w, const void *b, int wt, int bty,
+__global__ __launch_bounds__(columns_of(V)) void last_sums_kernel(Map x, Map dy, Shape sh, Cut cut, Between bt, const void *w, const void *b, int wt, int bty,
                                                         double2 *chan, double2 *group)
 {
     using R = typename T::raw;
@@ -243,11 +254,23 @@ __global__ __launch_bounds__(512) void last_sums_kernel(Map x, Map dy, Shape sh,
     }
     if (!group) return;                                                    // (uniform)
     __syncthreads();
-    for (int g = threadIdx.x; g < sh.G; g += T0) {
+    const int lanes = min(min(32, T0 / sh.G), (sh.cg + 15) / 16), g = threadIdx.x / lanes, l = threadIdx.x % lanes;     // of a group
+    if (g < sh.G) {
         double2 t = make_double2(0, 0);
-        for (int j = 0; j < sh.cg; j++) {
+        for (int j = l; j < sh.cg; j += lanes) {
             t.x += mine[g * sh.cg + j].x;
             t.y += mine[g * sh.cg + j].y;
+        }
+        if (lanes == 1) group[row * sh.G + g] = t;
+        else half[threadIdx.x] = t;
+    }
+    if (lanes == 1) return;
+    __syncthreads();
+    if (g < sh.G && l == 0) {
+        double2 t = half[threadIdx.x];
+        for (int i = 1; i < lanes; i++) {
+            t.x += half[threadIdx.x + i].x;
+            t.y += half[threadIdx.x + i].y;
         }
         group[row * sh.G + g] = t;
     }
@@ -256,11 +279,11 @@ __global__ __launch_bounds__(512) void last_sums_kernel(Map x, Map dy, Shape sh,
 constexpr int kJoinedGroups = 32;
 
 template <class T, int V, class OP>
-__global__ __launch_bounds__(512) void last_value_kernel(Map x, Map dy, Map out, Shape sh, Cut cut, Between bt, const void *w, const void *b, int wt, int bty)
+__global__ __launch_bounds__(columns_of(V)) void last_value_kernel(Map x, Map dy, Map out, Shape sh, Cut cut, Between bt, const void *w, const void *b, int wt, int bty)
 {
     using R = typename T::raw;
     extern __shared__ double lds[];
-    __shared__ double2 total[512];
+    __shared__ double2 total[columns_of(V)];
     __shared__ Stat stat[kJoinedGroups];
     if (OP::kTwo && blockIdx.x >= bt.blocks) {
         const int c = (blockIdx.x - bt.blocks) * (blockDim.x / 64) + threadIdx.x / 64;
@@ -498,9 +521,9 @@ Cut cut_of(int N, int C, int64_t S, int v, int workgroups, int64_t most, int *th
     const int g = gcd(C, v);
     c.rows = v / g;
     c.cols = C / g;
-    c.tiles = ceil_div(c.cols, 512);
+    c.tiles = ceil_div(c.cols, columns_of(v));
     c.tile = ceil_div(c.cols, c.tiles);
-    c.deep = (c.tile > 256 ? 512 : 256) / c.tile;
+    c.deep = c.tile > 512 ? 1 : (c.tile > 256 ? 512 : 256) / c.tile;
     *threads = (c.deep * c.tile + 63) / 64 * 64;
     c.periods = (S + c.rows - 1) / c.rows;
     const int64_t turns = (c.periods + c.deep - 1) / c.deep;
@@ -530,7 +553,7 @@ struct Call {
     size_t sums_lds(size_t coef) const
     {
         const int places = sums.tile * v, parts = places < threads ? threads / places : 1;
-        const size_t a = sizeof(double2) * (v * threads + parts * places), b = coef_bytes(sh, sums, v, coef);
+        const size_t a = sizeof(double2) * (v * threads + (parts * places > threads ? parts * places : threads)), b = coef_bytes(sh, sums, v, coef);
         return a > b ? a : b;
     }
 };
@@ -543,7 +566,7 @@ void cut_call(Call &c, int64_t N, int64_t C, int64_t S, int groups)
         const int64_t most = kJoined / groups > 64 ? kJoined / groups : 64;
         c.sums = cut_of((int)N, (int)C, S, c.v, kSumsLast, INT32_MAX, &c.threads);
         const int64_t turns = (c.sums.periods + c.sums.deep - 1) / c.sums.deep;
-        c.joined = c.sums.tiles == 1 && groups <= kJoinedGroups && C <= 512 && c.threads * c.v <= 2048 &&
+        c.joined = c.sums.tiles == 1 && groups <= kJoinedGroups &&
                    (c.sums.chunks <= most || N * most >= kSumsLast / 2 || turns <= kFew * most);
         if (c.joined) c.sums = cut_of((int)N, (int)C, S, c.v, kSumsLast, most, &c.threads);
         c.values = cut_of((int)N, (int)C, S, c.v, kValueWorkgroups, INT32_MAX, &c.threads);
