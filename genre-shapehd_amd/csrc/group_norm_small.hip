@@ -1,6 +1,6 @@
 // group_norm_small.hip -- group normalisation where one workgroup holds an image's group in its registers.
 //
-// A map whose groups hold up to 16384 values takes one launch, reads x (and dy) once, and needs no scratch.  A group is `rows` runs of `cols` accesses of V values: channels last, a run is one position's cg channels and every
+// A map whose groups hold up to 16384 values (backward: 8192 channels last, 4096 first) takes one launch, reads x (and dy) once, and needs no scratch.  A group is `rows` runs of `cols` accesses of V values: channels last, a run is one position's cg channels and every
 // thread keeps one column; channels first, a run is one channel's positions, shared by a team of 2^k threads.
 #include "group_norm.hpp"
 
@@ -9,7 +9,8 @@ namespace {
 
 using namespace gn;
 
-constexpr int kThreads = 1024, kValues = 16;                               // of the largest workgroup; of a thread
+// threads of the largest workgroup -- backward, whose columns' sums take 64 bytes of LDS a thread, fewer -- and values of a thread
+constexpr int kThreads = 1024, kBackwardThreads = 512, kValues = 16;
 
 struct Small {
     int rows, cols, team, deep, turns, subs;                               // threads of a run, runs at once, accesses of a thread and run, waves of a team
@@ -80,7 +81,7 @@ struct Walk {
 };
 
 template <class T, int V, bool LAST>
-__global__ __launch_bounds__(1024) void small_forward_kernel(Map x, Map y, Shape sh, Small m, double *stats, const void *w, const void *b, int wt, int bt)
+__global__ __launch_bounds__(kThreads) void small_forward_kernel(Map x, Map y, Shape sh, Small m, double *stats, const void *w, const void *b, int wt, int bt)
 {
     using R = typename T::raw;
     constexpr int K = kValues / V;
@@ -136,7 +137,7 @@ __global__ __launch_bounds__(1024) void small_forward_kernel(Map x, Map y, Shape
 
 // chan: the sums of dz and dz (x - mean) by image and channel (more than one image: added up behind this), or dw and db themselves
 template <class T, int V, bool LAST>
-__global__ __launch_bounds__(1024) void small_backward_kernel(Map x, Map dy, Map dx, Shape sh, Small m, const double *stats, const void *w, const void *b, int wt,
+__global__ __launch_bounds__(kBackwardThreads) void small_backward_kernel(Map x, Map dy, Map dx, Shape sh, Small m, const double *stats, const void *w, const void *b, int wt,
                                                              int bt, double2 *chan, void *dw, void *db)
 {
     using R = typename T::raw;
@@ -256,6 +257,7 @@ __global__ __launch_bounds__(1024) void small_backward_kernel(Map x, Map dy, Map
 // Values of a group, channels first, up to which the backward takes this form: with more (and with odd numbers of positions, whose
 // unrolled walk is 160 KB of code) the two-pass form is faster -- 4 x 160 x 8^3, 10240 values a group: 7.2 us against 12.3.
 constexpr int kBackwardFirst = 4096;
+constexpr int kMostChannels = 1024;                                        // of a group: its coefficients lie in LDS
 
 // the small form of a call, if its groups fit
 struct SmallCall { Small m; int v, threads; };
@@ -271,8 +273,8 @@ bool small_of(bool last, const Shape &sh, int es, bool backward, const Map &x, c
 {
     const int cg = sh.cg;
     const int64_t S = sh.S;
-    const int most = backward && !last ? kBackwardFirst : kThreads * kValues;
-    if (cg > 1024 || S > most || cg * S > most) return false;
+    const int threads = backward ? kBackwardThreads : kThreads, most = backward && !last ? kBackwardFirst : threads * kValues;
+    if (cg > kMostChannels || S > most || cg * S > most) return false;
     const int64_t run = last ? cg : S;
     // (run & 15 has run's powers of two up to 8; gcd(0, v) = v.)  Channels last, every value of a thread's column has sums of its own
     c.v = gcd((int)(run & 15), last ? 4 : 16 / es);
@@ -288,7 +290,7 @@ bool small_of(bool last, const Shape &sh, int es, bool backward, const Map &x, c
     m.gsd = cg * d.sc;
     m.gso = cg * out.sc;
     const int k = kValues / c.v;
-    for (c.threads = 64; c.threads <= kThreads; c.threads *= 2) {
+    for (c.threads = 64; c.threads <= threads; c.threads *= 2) {
         m.turns = m.subs = 1;
         if (last) {
             m.team = m.cols;
@@ -319,10 +321,9 @@ int forward_as(const Shape &sh, const SmallCall &k, const Map &x, const Map &y, 
 template <class T, int V, bool LAST>
 int backward_as(const Shape &sh, const SmallCall &k, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st)
 {
-    static std::atomic<uint64_t> reserved{0};
+    static_assert(8 * 3 * kMostChannels + 16 * 4 * kBackwardThreads + 512 <= 65536, "LDS of a launch");
     const bool one = sh.N == 1;
     const size_t lds = sizeof(double) * (3 * sh.cg + (sh.cg & 1)) + sizeof(double2) * (LAST ? V * k.threads : sh.cg * k.m.subs);
-    if (lds > 65536 - 512 && !reserve_lds("group_norm_backward", (const void *)small_backward_kernel<T, V, LAST>, 160 * 1024 - 512, reserved)) return 0;
     double2 *chan = !one && (g.dw || g.db) ? (double2 *)ws : nullptr;
     small_backward_kernel<T, V, LAST><<<sh.N * sh.G, k.threads, lds, st>>>(x, dy, g.dx, sh, k.m, stats, p.w, p.b, p.wt, p.bt, chan, one ? g.dw : nullptr, one ? g.db : nullptr);
     GENRE_LAUNCH_CHECK("group norm backward");

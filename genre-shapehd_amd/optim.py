@@ -9,7 +9,7 @@ class ClipAdam(torch.optim.Adam):
     torch.nn.utils.clip_grad_norm_(all parameters, max_grad_norm) had run before every step, in a few launches for the whole
     network: the gradients are read twice and never written.  The norm that a step found is left in `grad_norm`, on the GPU.
 
-    The moments are fp32 whatever the weights' type.  Parameters without a gradient are passed over, as they are there."""
+    Not for capture in a HIP graph: a replay would repeat the step that was captured, its count with it.  The moments are fp32 whatever the weights' type.  Parameters without a gradient are passed over, as they are there."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0, max_grad_norm=None, decoupled_weight_decay=False):
         if max_grad_norm is not None and not max_grad_norm >= 0:
@@ -34,6 +34,8 @@ class ClipAdam(torch.optim.Adam):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("ClipAdam: a step cannot be captured: its count of steps lives on the host")
         # what is stepped together: the same options and the same number of steps behind it (`step` tensors are shared by those)
         batches, every = [], []
         for group in self.param_groups:

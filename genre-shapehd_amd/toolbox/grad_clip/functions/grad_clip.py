@@ -53,7 +53,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
 def clip_adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled=False,
                     max_norm=None, norm_type=2.0, factor=None):
     """one Adam step on `params` in place, `exp_avgs` and `exp_avg_sqs` with them, as if clip_grads_(grads, max_norm, norm_type) had
-    run before -- without writing the gradients.  step counts from 1.  weight_decay is added to the gradient, or (decoupled) shrinks
+    run before -- without writing the gradients.  step counts from 1 (a captured call replays with the one it was given).  weight_decay is added to the gradient, or (decoupled) shrinks
     the weights by lr * weight_decay.  params[i] and grads[i] have one type and layout, the states are fp32 in that layout; no two
     tensors may overlap.  Returns the norm of the gradients before the clip (None without max_norm).
     factor (instead of max_norm): one fp32 value on the same GPU that the gradients are multiplied by -- for weights that are

@@ -139,9 +139,9 @@ def main(argv=None):
     ap.add_argument("--lr", type=float, default=1e-4)
     ap.add_argument("--w_gan_loss", type=float, default=1e-3)
     ap.add_argument("--chamfer_weight", type=float, default=0.0)
-    ap.add_argument("--clip_grad", type=float, default=None, help="bound on the norm of a network's gradients together (default: none)")
+    ap.add_argument("--clip_grad", type=float, default=None, help="bound on the norm of a network's gradients together (GPU; default: none)")
     ap.add_argument("--norm", choices=["batch", "group"], default="batch",
-                    help="normalisation of the trained 3-D network (shapehd: voxel decoder, wgangp: generator, genre: refiner)")
+                    help="normalisation of the trained 3-D network (shapehd: voxel decoder, wgangp: generator, genre: refiner; group: GPU)")
     ap.add_argument("--backend", default=None)
     ap.add_argument("--save", default=None)
     ap.add_argument("--resume", default=None)

@@ -81,6 +81,16 @@ def test_norms_at_the_ends_of_the_range(genre, dev):
         assert math.isnan(genre.grad_norm(ts, kind).item())
 
 
+def test_a_tensor_of_more_than_2_31_values(genre, dev):
+    n = 2 ** 31 + 12345
+    t = torch.full((n,), 2.0, dtype=torch.bfloat16, device=dev)
+    t[-1] = -5
+    want = math.sqrt(4.0 * (n - 1) + 25)
+    assert genre.grad_norm([t], math.inf).item() == 5
+    assert abs(genre.clip_grads_([t], want / 2).item() / want - 1) <= 2 * U          # a factor of 1/2 but for 1e-11
+    assert t[-1].item() == -2.5 and t[:-1].min().item() == t[:-1].max().item() == 1
+
+
 def factor64(norm, max_norm):
     return min(1.0, max_norm / (norm + 1e-6))
 

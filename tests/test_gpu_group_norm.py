@@ -319,6 +319,35 @@ def test_captured_and_replayed(genre, dev):
                 assert torch.equal(got, want[k])
 
 
+@pytest.mark.parametrize("last", (False, True), ids=("first", "last"))
+def test_maps_of_more_than_2_31_values(genre, dev, last):
+    """channels of +1 and -1: mean 0, deviation 1, so r = 1 / sqrt(1 + eps), y = +-r, dx = r (1 - r^2) dy for dy = x, dw = r S, db = +-S"""
+    s = 2 ** 30 + 40
+    x = torch.ones((1, s, 2) if last else (1, 2, s), dtype=torch.bfloat16, device=dev)
+    x = x.transpose(1, 2) if last else x
+    x[:, 1].neg_()
+    w, b = torch.ones(2, device=dev, requires_grad=True), torch.zeros(2, device=dev, requires_grad=True)
+    dy, leaf = x.clone(), x.requires_grad_(True)
+    y = genre.group_norm_act(leaf, 1, w, b, eps=0.25)
+    dx, dw, db = torch.autograd.grad(y, (leaf, w, b), dy)
+    r = 1 / math.sqrt(1.25)
+    for got, value in ((y.detach(), r), (dx, r * (1 - r * r))):
+        for c, sign in ((0, 1), (1, -1)):
+            lo, hi = got[0, c].min().item(), got[0, c].max().item()
+            assert lo == hi and abs(lo - sign * value) <= (2.0 ** -9 + U) * value
+    assert abs(dw[0].item() / (r * s) - 1) <= 2 * U and abs(dw[1].item() / (r * s) - 1) <= 2 * U
+    assert abs(db[0].item() / s - 1) <= 2 * U and abs(db[1].item() / s + 1) <= 2 * U
+
+
+def test_under_autocast(genre, dev):
+    """types are what is given: a bf16 map with fp32 parameters, inside autocast as outside"""
+    x, dy, w, b = make(dev, 2, 12, (5, 6), torch.bfloat16, True)
+    want = run(genre, x, dy, w, b, 3, "silu")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        got = run(genre, x, dy, w, b, 3, "silu")
+    assert all(torch.equal(got[k], want[k]) for k in want)
+
+
 def test_as_torch_has_it(genre, dev):
     """the layers that GroupNormAct replaces, in float64 (nn.GroupNorm behind a state_dict of the same keys)"""
     ours = genre.GroupNormAct(4, 20, act="leaky_relu", slope=0.01).to(dev)

@@ -179,6 +179,35 @@ def test_weights_that_a_graph_still_needs_are_seen_to_change(genre, dev):
         loss.backward()
 
 
+def test_a_step_is_not_captured(genre, dev):
+    p = torch.nn.Parameter(torch.ones(5, device=dev))
+    p.grad = torch.ones_like(p)
+    opt = genre.ClipAdam([p], max_grad_norm=1.0)
+    opt.step()
+    graph, kept = torch.cuda.CUDAGraph(), p.detach().clone()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(graph):
+            opt.step()
+    assert torch.equal(p, kept) and float(opt.state[p]["step"]) == 1
+
+
+def test_what_autograd_guards(genre, dev):
+    """a map changed between forward and backward raises; a result changed in place does not matter, as the map is what is kept;
+    a second backward through a retained graph gives the same"""
+    x, w = torch.randn(2, 8, 4, 4, device=dev, requires_grad=True), torch.ones(8, device=dev, requires_grad=True)
+    leaf = x * 1
+    y = genre.group_norm_act(leaf, 2, w, act="silu")
+    first = torch.autograd.grad(y.sum(), (x, w), retain_graph=True)
+    again = torch.autograd.grad(y.sum(), (x, w), retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(first, again))
+    z = y.mul_(2)
+    assert all(torch.equal(2 * a, b) for a, b in zip(first, torch.autograd.grad(z.sum(), (x, w), retain_graph=True)))
+    with torch.no_grad():
+        leaf.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 @pytest.mark.parametrize("config", ("shapehd", "wgangp", "genre"))
 def test_the_training_command(genre, dev, config, monkeypatch, capsys, tmp_path):
     """two steps of train.py with both options, on narrow networks (and without MIOpen's search, which takes minutes for new shapes)"""
