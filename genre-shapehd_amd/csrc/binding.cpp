@@ -11,6 +11,7 @@
 #include <vector>
 
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -73,6 +74,9 @@ int type_of(const Tensor &t)
     }
 }
 
+// uninitialised memory from torch's allocator, without the dispatcher's share of the call (a half of it)
+Tensor fresh(at::IntArrayRef size, at::ScalarType type, at::Device device) { return Tensor(at::detail::empty_cuda(size, type, device, std::nullopt)); }
+
 genre_tensor flat(const Tensor &t, int type)
 {
     genre_tensor d{};
@@ -110,22 +114,21 @@ Walk walk_of(const Tensor &t)
 // an uninitialised gap-free map in x's layout
 Tensor like(const Tensor &x, const Walk &w, Walk &out)
 {
-    Tensor y = at::empty_like(x);
-    out = walk_of(y);
-    if (out.ok && out.last == w.last) return y;
-    // (the order of x's dimensions is not one of the two: it has images or positions in another order, or expanded ones)
     const int64_t c = x.size(1), s = x.numel() / (x.size(0) * c);
-    std::vector<int64_t> size(x.sizes().begin(), x.sizes().end()), stride(size.size());
+    if (w.image == c * s && (w.last ? w.position == c : w.channel == s)) {
+        out = w;
+        return Tensor(at::detail::empty_strided_cuda(x.sizes(), x.strides(), x.scalar_type(), x.device()));
+    }
+    std::vector<int64_t> stride(x.dim());
     int64_t at = w.last ? c : 1;
     for (int64_t i = x.dim() - 1; i >= 2; i--) {
         stride[i] = at;
-        at *= size[i];
+        at *= x.size(i);
     }
     stride[0] = c * s;
     stride[1] = w.last ? 1 : s;
-    y = at::empty_strided(size, stride, x.options());
     out = {true, w.last, c * s, stride[1], w.last ? c : 1};
-    return y;
+    return Tensor(at::detail::empty_strided_cuda(x.sizes(), stride, x.scalar_type(), x.device()));
 }
 
 genre_tensor map(const Tensor &t, const Walk &w)
@@ -169,7 +172,7 @@ struct Scratch {
         const int64_t need = lib.gn_workspace(&x, (int)groups, backward);
         TORCH_CHECK(need >= 0, lib.last_error());
         if (!need) return;
-        keep = at::empty({need}, like.options().dtype(at::kDouble));
+        keep = fresh({need}, at::kDouble, like.device());
         d = flat(keep, GENRE_F64);
         arg = &d;
     }
@@ -178,7 +181,7 @@ struct Scratch {
 Forward gn_forward(const Tensor &given, const Tensor &weight, const Tensor &bias, int64_t groups, double eps, int64_t act, double slope)
 {
     const c10::DeviceGuard guard(given.device());
-    Forward f{given, {}, at::empty({2, given.size(0), groups}, given.options().dtype(at::kDouble))};
+    Forward f{given, {}, fresh({2, given.size(0), groups}, at::kDouble, given.device())};
     if (!given.numel()) {
         f.y = at::empty_like(given);
         return f;
@@ -221,8 +224,8 @@ public:
         Tensor dy = grads[0], dx, dw, db;
         const c10::DeviceGuard guard(x.device());
         // (the edges are those of the tensors that were given)
-        if (weight.defined() && ctx->needs_input_grad(1)) dw = at::empty_like(weight, at::MemoryFormat::Contiguous);
-        if (bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1)) db = at::empty_like(bias, at::MemoryFormat::Contiguous);
+        if (weight.defined() && ctx->needs_input_grad(1)) dw = fresh({x.size(1)}, weight.scalar_type(), x.device());
+        if (bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1)) db = fresh({x.size(1)}, bias.scalar_type(), x.device());
         if (!dy.defined()) dy = at::zeros_like(x);
         if (!x.numel()) {
             if (ctx->needs_input_grad(0)) dx = at::empty_like(x);
@@ -343,11 +346,10 @@ void bump(pybind11::handle list)
 
 Tensor norm_and_factor(const char *op, const Lists &l, int64_t kind, double max_norm)
 {
-    const auto options = at::TensorOptions().device(l.device);
-    Tensor out = at::empty({2}, options.dtype(at::kFloat));
+    Tensor out = fresh({2}, at::kFloat, l.device);
     const int64_t need = lib.grad_workspace(l.numel.data(), l.n());
     TORCH_CHECK(need >= 0, lib.last_error());
-    const Tensor ws = at::empty({need}, options.dtype(at::kDouble));
+    const Tensor ws = fresh({need}, at::kDouble, l.device);
     const genre_tensor o = flat(out, GENRE_F32), w = flat(ws, GENRE_F64);
     GENRE_CALL(op, lib.grad_norm(l.at[0].data(), l.numel.data(), l.type.data(), l.n(), (int)kind, (float)max_norm, &o, &w, stream_of(out)));
     return out;

@@ -8,8 +8,17 @@
 //
 // Sums and statistics are fp64 (gfx950 issues an fp64 FMA at the rate of an fp32 one, and the passes wait for memory) and taken of
 // x less its group's first value, so that sum x^2 / M - mean^2 cancels nothing where the mean is many deviations from zero; z's
-// sign -- which side of its jump a ReLU's derivative takes -- is that of the exact z.  y and dx are rounded once, to their type.  No atomics: partial sums lie in the workspace and are added
-// in a fixed order, so a call's result depends on nothing but its inputs.
+// sign -- which side of its jump a ReLU's derivative takes -- is that of the exact z.  y and dx are rounded once, to their type.
+// No atomics: partial sums lie in the workspace and are added in a fixed order, so a call's result depends on nothing but its inputs.
+//
+// Groups of up to 16384 values are group_norm_small.hip's.  Here a map takes two passes, each a launch: sums (by chunk of an image
+// and channel, in the workspace), then values, whose workgroups first add up their groups' chunks -- a launch of its own between
+// the passes cost 5 to 9 us.  What is read twice is the price: an image's group does not fit a CU, and a wait of workgroups for one
+// another inside a launch would need all of them resident.  Bound: HBM, at what a copy reaches (4.9 to 5.3 TB/s) or above it,
+// where the second pass, which starts where the first ended, still finds x in the 256 MB cache.  Measured:
+//   4 x 20 x 64^3 fp32 channels last, leaky ReLU: forward 17 + 31 us (84 MB read, 84 MB read + 86 written), backward 29 + 44 us
+//   8 x 32 x 64^3 bf16 channels first, ReLU:      forward 23 + 42 us (134 MB,       134 + 134),            backward 41 + 61 us
+// y and dx are stored past the caches: a launch's end waits for what it left dirty in the L2s (58.7 -> 47.4 us and 88.8 -> 73.4).
 #include "group_norm.hpp"
 
 namespace genre {
@@ -505,8 +514,9 @@ int width_of(const genre_tensor *x, bool last, bool dense)
 // reduction by column, 47.4 / 51.3 us (training 126 / 137); decoder 64^3 x8, channels first, 73.5 / 71.3 (179 / 175).  Values 2048 /
 // 4096: 47.4 / 47.4 and 73.5 / 72.0 (126.1 / 125.9 and 179.5 / 177.2).
 constexpr int kSumsLast = 1024, kSumsFirst = 2048, kValueWorkgroups = 4096;
-constexpr int kFew = 32;
-constexpr int kJoined = 1024;                                              // pairs that a workgroup of the second pass adds up itself
+// Pairs that a workgroup of the second pass adds up itself (16 KB from the caches; 2048: 4 x 40 x 32^3 backward 26 -> 30 us), and
+// accesses of a thread of the first pass beyond which more chunks and a launch between the passes are faster.
+constexpr int kJoined = 1024, kFew = 32;
 
 int chunks_of(int64_t turns, int64_t others, int workgroups, int64_t most)
 {
