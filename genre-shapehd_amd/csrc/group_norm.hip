@@ -122,7 +122,7 @@ struct SumsB {                                                             // dz
     __device__ static Coef coef(double, const Stat &t, float w, float b) { return {t.mean, t.r * w, b}; }
     __device__ static void add(const Coef &k, float slope, float x, float dy, double &s, double &q)
     {
-        const double d = (double)x - k.mean, dz = dy * act_slope<ACT>(fma(d, k.a, k.b), slope);
+        const double d = (double)x - k.mean, dz = act_grad<ACT>(fma(d, k.a, k.b), dy, slope);
         s += dz;
         q = fma(dz, d, q);
     }
@@ -141,7 +141,7 @@ struct ValueB {
     __device__ static Coef coef(const Stat &t, float w, float b) { return {t.mean, t.r * w, b, t.r * t.m1, t.r * t.r * t.m2}; }
     __device__ static float value(const Coef &k, float slope, float x, float dy)
     {
-        const double d = (double)x - k.mean, dz = dy * act_slope<ACT>(fma(d, k.a, k.b), slope);
+        const double d = (double)x - k.mean, dz = act_grad<ACT>(fma(d, k.a, k.b), dy, slope);
         return (float)fma(dz, k.a, -fma(d, k.k3, k.k2));
     }
 };

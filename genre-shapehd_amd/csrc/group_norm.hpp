@@ -81,16 +81,17 @@ __device__ __forceinline__ float act_value(double z, float slope)
     if (ACT == kActSilu) return f * sigmoid(f);
     return f;
 }
+// dz of dy.  A ReLU that is off passes nothing on, whatever dy holds there (an infinity times 0 would be a NaN)
 template <int ACT>
-__device__ __forceinline__ float act_slope(double z, float slope)
+__device__ __forceinline__ float act_grad(double z, float dy, float slope)
 {
-    if (ACT == kActRelu) return z > 0 ? 1.f : 0.f;
-    if (ACT == kActLeaky) return z > 0 ? 1.f : slope;
+    if (ACT == kActRelu) return z > 0 ? dy : 0.f;
+    if (ACT == kActLeaky) return z > 0 ? dy : dy * slope;
     if (ACT == kActSilu) {
         const float f = (float)z, s = sigmoid(f);
-        return s * fmaf(f, 1.f - s, 1.f);
+        return dy * (s * fmaf(f, 1.f - s, 1.f));
     }
-    return 1.f;
+    return dy;
 }
 
 // ---- what the kernels know of a call ----------------------------------------------------------------------------

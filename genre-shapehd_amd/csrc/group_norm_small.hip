@@ -181,7 +181,7 @@ __global__ __launch_bounds__(kBackwardThreads) void small_backward_kernel(Map x,
 #pragma unroll
                 for (int i = 0; i < V; i++) {
                     const int e = LAST ? i : 0;
-                    const double h = (double)v[k].at(i) - mean, dz = d[k].at(i) * act_slope<act>(fma(h, coef[c + e], coef[cg + c + e]), sh.slope);
+                    const double h = (double)v[k].at(i) - mean, dz = act_grad<act>(fma(h, coef[c + e], coef[cg + c + e]), d[k].at(i), sh.slope);
                     acc[e].x += dz;
                     acc[e].y = fma(dz, h, acc[e].y);
                 }
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kBackwardThreads) void small_backward_kernel(Map x,
 #pragma unroll
                 for (int i = 0; i < V; i++) {
                     const int e = LAST ? i : 0;
-                    const double h = (double)v[k].at(i) - mean, dz = d[k].at(i) * act_slope<act>(fma(h, coef[c + e], coef[cg + c + e]), sh.slope);
+                    const double h = (double)v[k].at(i) - mean, dz = act_grad<act>(fma(h, coef[c + e], coef[cg + c + e]), d[k].at(i), sh.slope);
                     f[i] = (float)fma(dz, coef[c + e], -fma(h, k3, k2));
                 }
                 store<T, V>(po + at.row * m.pso + at.col * V, f);

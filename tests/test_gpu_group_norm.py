@@ -249,6 +249,19 @@ def test_one_bad_value_spoils_its_group_only(genre, dev, bad, last):
         assert torch.equal(got[k][[0, 1, 4, 5, 6, 7, 8, 9]], clean[k][[0, 1, 4, 5, 6, 7, 8, 9]])
 
 
+@pytest.mark.parametrize("bad", (math.nan, math.inf, -math.inf))
+@pytest.mark.parametrize("last", (False, True), ids=("first", "last"))
+def test_a_relu_that_is_off_passes_nothing_on(genre, dev, bad, last):
+    """whatever the gradient holds there: the same bits as with zeros in its place (one workgroup a group, and two passes)"""
+    for space in ((5, 9), (90, 91)):
+        x, dy, w, b = make(dev, 2, 8, space, torch.float32, last)
+        off = run(genre, x, dy, w, b, 2, "relu")["y"] == 0
+        want = run(genre, x, dy.masked_fill(off, 0.0), w, b, 2, "relu")
+        got = run(genre, x, dy.masked_fill(off, bad), w, b, 2, "relu")
+        for k in got:
+            assert bool(got[k].isfinite().all()) and torch.equal(got[k], want[k])
+
+
 def test_gradients_against_differences(genre, dev):
     """the smooth activation, central differences of the operator's own fp32 forward summed in float64: the step h = 2^-6 leaves a
     truncation of h^2 / 6 times the third derivative of the loss (below 40 here: |r| <= 4, |dy| <= 3, few terms) = 2e-3 and a rounding of
