@@ -717,6 +717,13 @@ int backward(const Call &c, const Map &x, const Map &dy, const Params &p, const 
 
 #define GENRE_BY_WIDTH(T, v, call8, call4, call2, call1) ((v) == 8 ? call8 : (v) == 4 ? call4 : (v) == 2 ? call2 : call1)
 
+// scratch of a call whose maps all lie as `c` says
+int64_t needed(const Call &c, const genre_tensor *x, bool backward)
+{
+    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, backward)) return backward ? small_workspace(c.sh) : 0;
+    return workspace_of(c, backward);
+}
+
 }  // namespace
 }  // namespace genre
 
@@ -729,14 +736,17 @@ extern "C" int64_t genre_group_norm_workspace(const genre_tensor *x, int groups,
     if (!x) { fail("%s: x is NULL", op); return -1; }
     if (!check_map(op, "x", x, x) || !plan(op, x, nullptr, 0, groups, c)) return -1;
     if (numel(x) == 0) return 0;
-    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, backward != 0)) return backward ? small_workspace(c.sh) : 0;
-    int64_t need = workspace_of(c, backward != 0);
-    if (c.last) {                                                          // a gap in another map's rows narrows the columns: room for both
+    int64_t need = needed(c, x, backward != 0);
+    // the other maps may make another call of it: gaps in their rows narrow the columns, and with one position (which lies in both
+    // ways) they may leave channels first only.  Room for all
+    for (int other = 0; other < 2 && c.last; other++) {
+        if (other && !channels_first(x)) continue;
         Call d = c;
-        d.v = width_of(x, true, false);
+        d.last = !other;
+        d.v = width_of(x, d.last, false);
         cut_call(d, d.sh.N, d.sh.C, d.sh.S, groups);
-        const int64_t other = workspace_of(d, backward != 0);
-        if (other > need) need = other;
+        const int64_t n = needed(d, x, backward != 0);
+        if (n > need) need = n;
     }
     return need;
 }

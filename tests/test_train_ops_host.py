@@ -74,6 +74,17 @@ def test_group_norm_entries(lib):
     assert lib.genre_group_norm_workspace(desc(L, (2, 6, 50000)), 2, 0) > 0
 
 
+@pytest.mark.parametrize("dtype", (0, 2))
+@pytest.mark.parametrize("n,c,groups", ((1, 16, 4), (1, 640, 8), (2, 16, 4), (3, 5000, 2), (1, 20000, 1), (2, 40000, 2), (1, 70000, 2), (5, 99999, 3)))
+def test_scratch_of_one_position_serves_both_layouts(lib, n, c, groups, dtype):
+    """a [N, C, 1] map is channels last and channels first at once; which of them a call is, the other maps may decide"""
+    L, lib = lib
+    need = lambda stride, back: lib.genre_group_norm_workspace(desc(L, (n, c, 1), stride=stride, dtype=dtype), C.c_int(groups), C.c_int(back))
+    for back in (0, 1):
+        both, first = need((c, 1, 1), back), need((2 * c, 2, 1), back)
+        assert both >= first >= 0
+
+
 def test_list_entries(lib):
     L, lib = lib
     i64, i32, ptr = lambda *v: (C.c_int64 * len(v))(*v), lambda *v: (C.c_int32 * len(v))(*v), lambda *v: (C.c_void_p * len(v))(*v)
