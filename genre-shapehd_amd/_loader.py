@@ -326,7 +326,7 @@ class _TrainingLib:
         mod = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(mod)
         mod.bind_library(LIB_PATH)
-        for fn in ("group_norm_act", "grad_norm", "clip_grads", "adam_step"):
+        for fn in ("group_norm_act", "grad_norm", "clip_grads", "adam_step", "laid_otherwise"):
             self.__dict__[fn] = getattr(mod, fn)
         if name not in self.__dict__:
             raise AttributeError(name)

@@ -335,6 +335,25 @@ Lists first_list(const char *op, pybind11::handle list, bool written)
     return l;
 }
 
+// whether t's values lie in memory as those of the gap-free p do (a dimension of one value may have any stride)
+bool lies_as(const Tensor &t, const Tensor &p)
+{
+    if (t.sizes() != p.sizes()) return false;
+    if (t.is_contiguous() && p.is_contiguous()) return true;
+    for (int64_t i = 0; i < t.dim(); i++)
+        if (t.size(i) != 1 && t.stride(i) != p.stride(i)) return false;
+    return true;
+}
+
+// the places at which `others` does not lie as `weights` (of the same length)
+std::vector<int64_t> laid_otherwise(pybind11::handle weights, pybind11::handle others)
+{
+    std::vector<int64_t> at;
+    for (Py_ssize_t i = 0, n = PySequence_Fast_GET_SIZE(weights.ptr()); i < n; i++)
+        if (!lies_as(item("laid_otherwise", others.ptr(), i), item("laid_otherwise", weights.ptr(), i))) at.push_back(i);
+    return at;
+}
+
 void bump(pybind11::handle list)
 {
     PyObject *p = list.ptr();
@@ -392,8 +411,8 @@ OptTensor adam_step(pybind11::handle params, pybind11::handle grads, pybind11::h
             const Tensor &p = THPVariable_Unpack(PySequence_Fast_GET_ITEM(params.ptr(), i)), &t = item(op, more[k].ptr(), i);
             TORCH_CHECK(t.device() == l.device && t.layout() == at::kStrided && t.scalar_type() == (k ? at::kFloat : p.scalar_type()), op, ": ", names[k], " ", i, " is ",
                         t.scalar_type(), " ", t.layout(), " on ", t.device(), " for ", p.scalar_type(), " on ", l.device, " (", k ? "fp32 is wanted" : "the same is wanted", ")");
-            TORCH_CHECK(t.sizes() == p.sizes() && (t.strides() == p.strides() || (t.is_contiguous() && p.is_contiguous())), op, ": ", names[k], " ", i, " ",
-                        t.sizes(), " with strides ", t.strides(), " does not lie as its weight ", p.sizes(), " with strides ", p.strides());
+            TORCH_CHECK(lies_as(t, p), op, ": ", names[k], " ", i, " ", t.sizes(), " with strides ", t.strides(), " does not lie as its weight ", p.sizes(),
+                        " with strides ", p.strides());
             at[i] = t.data_ptr();
         }
         l.at.push_back(std::move(at));
@@ -431,4 +450,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m)
     m.def("grad_norm", &grad_norm);
     m.def("clip_grads", &clip_grads);
     m.def("adam_step", &adam_step);
+    m.def("laid_otherwise", &laid_otherwise);
 }

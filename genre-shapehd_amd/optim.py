@@ -59,6 +59,12 @@ class ClipAdam(torch.optim.Adam):
             self.grad_norm, factor = _native.grad_norm(every, float(self.max_grad_norm), 2)
         for group, count, members in batches:
             params, grads, states = zip(*members)
+            params, grads = list(params), list(grads)
+            for i in _native.laid_otherwise(params, grads):
+                grads[i] = torch.empty_like(params[i]).copy_(grads[i])
+            for name in ("exp_avg", "exp_avg_sq"):                     # (moments of weights whose layout has changed, or loaded ones)
+                for i in _native.laid_otherwise(params, [s[name] for s in states]):
+                    states[i][name] = torch.empty_like(params[i], dtype=torch.float32).copy_(states[i][name])
             clip_adam_step_(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], count + 1, lr=float(group["lr"]),
                             betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                             decoupled=group.get("decoupled_weight_decay", False), factor=factor)

@@ -221,6 +221,18 @@ def test_layouts_of_weights_and_states(genre, dev):
         genre.clip_grads_([torch.ones(10, device=dev)[::2]], 1.0)
 
 
+def test_strides_of_dimensions_of_one_value_do_not_matter(genre, dev):
+    """the gradient of a channels-last weight with one output channel may come with any stride there"""
+    p, g = (torch.randn(1, 8, 4, 4, 4, device=dev).to(memory_format=torch.channels_last_3d) for _ in range(2))
+    m, v, q = torch.zeros_like(p), torch.zeros_like(p), p.clone()
+    other = g.as_strided(g.shape, (1, *g.stride()[1:]))
+    assert other.stride() != p.stride() and torch.equal(other, g)
+    a, b = torch.zeros_like(q), torch.zeros_like(q)
+    genre.clip_adam_step_([p], [other], [m], [v], 1, max_norm=1.0)
+    genre.clip_adam_step_([q], [g], [a], [b], 1, max_norm=1.0)
+    assert torch.equal(p, q) and torch.equal(m, a) and torch.equal(v, b)
+
+
 def test_refusals(genre, dev):
     t, s = [torch.zeros(4, device=dev)], [torch.zeros(4, device=dev)]
     for bad in (lambda: genre.grad_norm(t, 1.0), lambda: genre.grad_norm([torch.zeros(3)]), lambda: genre.grad_norm([t[0].double()]),

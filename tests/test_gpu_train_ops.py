@@ -155,6 +155,31 @@ def test_states_go_to_torch_and_back(genre, dev, tmp_path):
         assert all(st["exp_avg"].dtype == torch.float32 and float(st["step"]) == 2 for st in third.state.values())
 
 
+def test_gradients_and_moments_in_another_layout(genre, dev):
+    """the same bits (no bound: no sum whose order a layout changes) when gradients, or weights after the first step, change it"""
+    def build():
+        torch.manual_seed(5)
+        ps = [torch.nn.Parameter(torch.randn(s, device=dev)) for s in ((6, 5, 4, 4, 4), (1, 3, 2, 2, 2), (7,))]
+        return ps, genre.ClipAdam(ps, lr=1e-2)
+
+    last = lambda t: t.to(memory_format=torch.channels_last_3d) if t.dim() == 5 else t
+    plain, opt = build()
+    other, opt2 = build()
+    for step in range(3):
+        g = torch.Generator().manual_seed(step)
+        if step == 1:
+            for p in other:
+                p.data = last(p.data)
+        for p, q in zip(plain, other):
+            p.grad = torch.randn(p.shape, generator=g).to(dev)
+            q.grad = p.grad.clone() if step == 2 else last(p.grad)
+        opt.step()
+        opt2.step()
+        assert all(torch.equal(p, q) for p, q in zip(plain, other))
+        assert all(torch.equal(opt.state[p][k], opt2.state[q][k]) for p, q in zip(plain, other) for k in ("exp_avg", "exp_avg_sq"))
+    assert other[0].is_contiguous(memory_format=torch.channels_last_3d) and opt2.state[other[0]]["exp_avg"].stride() == other[0].stride()
+
+
 def test_a_step_without_a_bound_and_one_without_gradients(genre, dev):
     ps = weights(dev, 2)
     opt = genre.ClipAdam(ps, lr=1e-2)
