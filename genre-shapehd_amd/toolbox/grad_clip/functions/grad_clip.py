@@ -31,7 +31,7 @@ def _bound(op, max_norm):
 
 def grad_norm(tensors, norm_type=2.0):
     """norm of the vector of all the tensors' values (2: Euclidean, fp64 sums; inf: the largest magnitude) as an fp32 tensor of no
-    dimensions on their GPU.  NaN where a value is NaN.  An empty list has the norm 0 (on the CPU, as nothing names a GPU)."""
+    dimensions on their GPU.  NaN where a value is NaN.  It carries no gradient.  An empty list has the norm 0 (on the CPU, as nothing names a GPU)."""
     kind, tensors = _kind("grad_norm", norm_type), _list(tensors)
     return _native.grad_norm(tensors, math.inf, kind)[0] if tensors else torch.tensor(0.0)
 
@@ -39,7 +39,7 @@ def grad_norm(tensors, norm_type=2.0):
 def clip_grads_(tensors, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """scale the tensors in place by min(1, max_norm / (norm + 1e-6)), norm = grad_norm(tensors, norm_type), and return the norm.
     A norm of infinity scales by 0 (infinities become NaN), NaN makes all NaN; error_if_nonfinite raises before anything is
-    written instead, for which it waits for the GPU.  No two tensors may overlap."""
+    written instead, for which it waits for the GPU.  Tensors that share memory, or one that is listed twice, are refused."""
     kind, max_norm, tensors = _kind("clip_grads_", norm_type), _bound("clip_grads_", max_norm), _list(tensors)
     return _native.clip_grads(tensors, max_norm, kind, error_if_nonfinite) if tensors else torch.tensor(0.0)
 
@@ -53,9 +53,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
 def clip_adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, decoupled=False,
                     max_norm=None, norm_type=2.0, factor=None):
     """one Adam step on `params` in place, `exp_avgs` and `exp_avg_sqs` with them, as if clip_grads_(grads, max_norm, norm_type) had
-    run before -- without writing the gradients.  step counts from 1 (a captured call replays with the one it was given).  weight_decay is added to the gradient, or (decoupled) shrinks
-    the weights by lr * weight_decay.  params[i] and grads[i] have one type and layout, the states are fp32 in that layout; no two
-    tensors may overlap.  Returns the norm of the gradients before the clip (None without max_norm).
+    run before -- without writing the gradients.  step counts from 1 (a captured call replays with the one it was given).
+    weight_decay is added to the gradient, or (decoupled) shrinks the weights by lr * weight_decay.  params[i] and grads[i] have one type and layout, the states are fp32 in that layout;
+    tensors that share memory are refused (gradients may, with each other).  Returns the norm of the gradients before the clip (None without max_norm).
     factor (instead of max_norm): one fp32 value on the same GPU that the gradients are multiplied by -- for weights that are
     stepped in several calls under one clip."""
     kind = _kind("clip_adam_step_", norm_type)

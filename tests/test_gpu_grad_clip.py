@@ -245,6 +245,26 @@ def test_refusals(genre, dev):
             bad()
 
 
+def test_tensors_that_share_memory_are_refused(genre, dev):
+    """before anything is written; gradients may be the same tensor, as nothing writes them"""
+    flat = torch.ones(5000, device=dev)
+    a, b = flat[:3000], flat[2999:]
+    for ts in ([a, b], [b, a], [a, a], [flat, flat[7:8]], [a, flat[3000:], a.view(60, 50)]):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            genre.clip_grads_(ts, 1.0)
+    p, m, v = (tensors(dev, [(3000,), (3000,)], seed=s, scale=0.1) for s in (1, 2, 3))
+    v = [t.abs() for t in v]
+    g = tensors(dev, [(3000,)], seed=4)
+    kept = [t.clone() for t in p + m + v]
+    for lists in (([p[0], p[0]], g * 2, m, v), (p, g * 2, [m[0]] * 2, v), (p, g * 2, m, m), (p, [g[0], p[0]], m, v), (p, g * 2, m, [v[0], m[1]])):
+        with pytest.raises(RuntimeError, match="shares memory"):
+            genre.clip_adam_step_(*lists, 1, max_norm=1.0)
+    assert bool((flat == 1).all()) and all(torch.equal(t, k) for t, k in zip(p + m + v, kept))
+    genre.clip_grads_([flat[:3000], flat[3000:], flat[9:9]], 1e9)
+    genre.clip_adam_step_(p, g * 2, m, v, 1)
+    assert not torch.equal(p[0], kept[0])
+
+
 def test_streams_and_graphs(genre, dev):
     """captured norm + clip and clip + Adam, replayed with eager work and synchronisations between: the same bits as eager calls"""
     sizes = LISTS["odd"] + LISTS["many"][:250]
