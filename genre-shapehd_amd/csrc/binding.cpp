@@ -78,6 +78,9 @@ int type_of(const Tensor &t)
 // uninitialised memory from torch's allocator, without the dispatcher's share of the call (a half of it)
 Tensor fresh(at::IntArrayRef size, at::ScalarType type, at::Device device) { return Tensor(at::detail::empty_cuda(size, type, device, std::nullopt)); }
 
+// its values as they lie in memory (a view may hold the negatives of them)
+Tensor plain(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 genre_tensor flat(const Tensor &t, int type)
 {
     genre_tensor d{};
@@ -227,7 +230,7 @@ public:
         // (the edges are those of the tensors that were given)
         if (weight.defined() && ctx->needs_input_grad(1)) dw = fresh({x.size(1)}, weight.scalar_type(), x.device());
         if (bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1)) db = fresh({x.size(1)}, bias.scalar_type(), x.device());
-        if (!dy.defined()) dy = at::zeros_like(x);
+        dy = dy.defined() ? plain(dy) : at::zeros_like(x);
         if (!x.numel()) {
             if (ctx->needs_input_grad(0)) dx = at::empty_like(x);
             if (dw.defined()) dw.zero_();
@@ -270,9 +273,9 @@ void check_param(const char *what, const Tensor &t, const Tensor &x)
                 " must be a [", x.size(1), "] tensor of fp32, bf16 or fp16 on ", x.device(), ", got ", t.sizes(), " ", t.scalar_type(), " on ", t.device());
 }
 
-Tensor group_norm_act(const Tensor &x, int64_t groups, const OptTensor &weight, const OptTensor &bias, double eps, int64_t act, double slope)
+Tensor group_norm_act(const Tensor &given, int64_t groups, const OptTensor &weight, const OptTensor &bias, double eps, int64_t act, double slope)
 {
-    const Tensor w = weight.value_or(Tensor()), b = bias.value_or(Tensor());
+    const Tensor x = plain(given), w = weight ? plain(*weight) : Tensor(), b = bias ? plain(*bias) : Tensor();
     TORCH_CHECK(x.is_cuda(), "group_norm_act: x is on ", x.device(), "; GPU tensors only -- there is no CPU path");
     TORCH_CHECK(type_of(x) >= 0 && x.layout() == at::kStrided, "group_norm_act: ", x.scalar_type(), " ", x.layout(), " not supported (dense fp32, bf16 or fp16)");
     TORCH_CHECK(x.dim() >= 2, "group_norm_act: x must be [N, C, ...], got ", x.sizes());
@@ -280,9 +283,10 @@ Tensor group_norm_act(const Tensor &x, int64_t groups, const OptTensor &weight, 
     TORCH_CHECK(eps > 0, "group_norm_act: eps must be positive, got ", eps);
     check_param("weight", w, x);
     check_param("bias", b, x);
+    for (const Tensor &t : {x, w, b}) TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "group_norm_act: forward-mode derivatives are not supported");
     if (at::GradMode::is_enabled() && (x.requires_grad() || (w.defined() && w.requires_grad()) || (b.defined() && b.requires_grad()))) {
         pybind11::gil_scoped_release no_gil;
-        return GroupNormAct::apply(x, weight, bias, groups, eps, act, slope);
+        return GroupNormAct::apply(x, w.defined() ? OptTensor(w) : std::nullopt, b.defined() ? OptTensor(b) : std::nullopt, groups, eps, act, slope);
     }
     pybind11::gil_scoped_release no_gil;
     const at::AutoDispatchBelowADInplaceOrView below;
@@ -307,7 +311,7 @@ const Tensor &item(const char *op, PyObject *list, Py_ssize_t i)
     return THPVariable_Unpack(o);
 }
 
-bool gap_free(const Tensor &t) { return t.is_contiguous() || t.is_non_overlapping_and_dense(); }
+bool gap_free(const Tensor &t) { return !t.is_neg() && (t.is_contiguous() || t.is_non_overlapping_and_dense()); }
 
 // the first list: any gap-free tensors of one GPU and of the three types; others are refused where they are `written`, else copied
 Lists first_list(const char *op, pybind11::handle list, bool written)
@@ -329,8 +333,8 @@ Lists first_list(const char *op, pybind11::handle list, bool written)
             l.at[0][i] = t.data_ptr();
             continue;
         }
-        TORCH_CHECK(!written, op, ": tensor ", i, " ", t.sizes(), " with strides ", t.strides(), " has gaps or overlaps and cannot be written in place");
-        l.copies.push_back(t.detach().contiguous());
+        TORCH_CHECK(!written, op, ": tensor ", i, " ", t.sizes(), " with strides ", t.strides(), " has gaps or overlaps, or is a view of negatives, and cannot be written in place");
+        l.copies.push_back(plain(t.detach()).contiguous());
         l.at[0][i] = l.copies.back().data_ptr();
     }
     return l;
@@ -339,7 +343,7 @@ Lists first_list(const char *op, pybind11::handle list, bool written)
 // whether t's values lie in memory as those of the gap-free p do (a dimension of one value may have any stride)
 bool lies_as(const Tensor &t, const Tensor &p)
 {
-    if (t.sizes() != p.sizes()) return false;
+    if (t.sizes() != p.sizes() || t.is_neg()) return false;
     if (t.is_contiguous() && p.is_contiguous()) return true;
     for (int64_t i = 0; i < t.dim(); i++)
         if (t.size(i) != 1 && t.stride(i) != p.stride(i)) return false;

@@ -233,6 +233,44 @@ def test_what_autograd_guards(genre, dev):
         y.sum().backward()
 
 
+def test_views_of_negatives(genre, dev):
+    """torch's lazy negation (of a conjugate's imaginary part) is a flag on the tensor, not in its memory"""
+    x, dy, w = (torch.randn(s, device=dev) for s in ((2, 8, 4, 4), (2, 8, 4, 4), (8,)))
+    neg = lambda t: torch._neg_view(-t)
+
+    def run(x, dy, w):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, w)]
+        y = genre.group_norm_act(leaves[0], 2, leaves[1], act="silu")
+        return [y.detach(), *torch.autograd.grad(y, leaves, dy)]
+
+    want = run(x, dy, w)
+    assert neg(x).is_neg() and torch.equal(neg(x), x)
+    assert torch.equal(genre.group_norm_act(neg(x), 2, neg(w), act="silu"), want[0])
+    assert all(torch.equal(a, b) for a, b in zip(run(x, neg(dy), w), want))
+    leaf = x.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(genre.group_norm_act(torch._neg_view(leaf), 2, w, act="silu"), leaf, dy)[0], -run(-x, dy, w)[1])
+    assert genre.grad_norm([neg(x), dy]).item() == genre.grad_norm([x, dy]).item()
+    with pytest.raises(RuntimeError):
+        genre.clip_grads_([neg(x)], 1e-3)
+    m, v, p, q = torch.zeros_like(x), torch.zeros_like(x), torch.nn.Parameter(x.clone()), torch.nn.Parameter(x.clone())
+    with pytest.raises(RuntimeError):
+        genre.clip_adam_step_([p.detach()], [neg(dy)], [m], [v], 1)
+    for t, g in ((p, dy), (q, neg(dy))):
+        t.grad = g
+        genre.ClipAdam([t], max_grad_norm=1.0).step()
+    assert torch.equal(p, q)
+
+
+def test_forward_mode_is_refused(genre, dev):
+    """rather than a result without its tangent"""
+    from torch.autograd import forward_ad
+    x, w = torch.randn(2, 8, 4, device=dev), torch.randn(8, device=dev)
+    with forward_ad.dual_level():
+        for args in ((forward_ad.make_dual(x, x), 2), (x, 2, forward_ad.make_dual(w, w)), (x, 2, w, forward_ad.make_dual(w, w))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                genre.group_norm_act(*args)
+
+
 @pytest.mark.parametrize("config", ("shapehd", "wgangp", "genre"))
 def test_the_training_command(genre, dev, config, monkeypatch, capsys, tmp_path):
     """two steps of train.py with both options, on narrow networks (and without MIOpen's search, which takes minutes for new shapes)"""
