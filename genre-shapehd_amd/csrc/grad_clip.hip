@@ -164,7 +164,8 @@ struct Adam { float b1, c1, b2, c2, eps, step_size, inv_root_c2, decay, keep; };
 
 __device__ __forceinline__ void adam_value(const Adam &k, float f, float &p, float g, float &m, float &v)
 {
-    g = fmaf(k.decay, p, g * f);
+    g *= f;
+    if (k.decay != 0.f) g = fmaf(k.decay, p, g);                           // (0 times an infinite weight would be a NaN)
     m = fmaf(k.c1, g, k.b1 * m);
     v = fmaf(k.c2 * g, g, k.b2 * v);
     p = fmaf(-k.step_size, m / fmaf(sqrtf(v), k.inv_root_c2, k.eps), p * k.keep);

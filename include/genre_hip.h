@@ -477,7 +477,7 @@ int genre_group_norm_backward(const genre_tensor *x, const genre_tensor *dy, con
  *     0: the largest magnitude (NaN if one is) -- and the factor min(1, max_norm / (norm + 1e-6)) (NaN stays NaN; 1 for
  *     max_norm = infinity).  ws: fp64 scratch of at least genre_grad_workspace(numels, n) values.
  *   genre_grad_scale: every value times factor[0] (fp32, on the device), rounded to its type; 1 leaves the memory untouched
- *   genre_adam_step: with g' = g factor[0] + weight_decay p (factor NULL: 1; decoupled != 0: p is scaled by 1 - lr weight_decay
+ *   genre_adam_step: with g' = g factor[0] + weight_decay p (factor NULL: 1; weight_decay 0: g factor[0], whatever p; decoupled != 0: p is scaled by 1 - lr weight_decay
  *     instead),  m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2,
  *     p -= lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps);  p and g of dtypes[i], m and v fp32; g is not written. */
 int64_t genre_grad_workspace(const int64_t *numels, int n);

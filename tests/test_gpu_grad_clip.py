@@ -233,6 +233,21 @@ def test_strides_of_dimensions_of_one_value_do_not_matter(genre, dev):
     assert torch.equal(p, q) and torch.equal(m, a) and torch.equal(v, b)
 
 
+def test_weights_that_are_no_numbers_keep_their_moments_clean(genre, dev):
+    """without weight decay a gradient does not depend on its weight; an infinite weight stays one"""
+    for dtype in TYPES:
+        p, g = tensors(dev, [(37,)], dtype, 1)[0], tensors(dev, [(37,)], dtype, 2)[0]
+        q = p.clone()
+        p[3], p[36], p[20] = math.inf, -math.inf, math.nan
+        a, b, c, d = (torch.zeros(37, device=dev) for _ in range(4))
+        genre.clip_adam_step_([p], [g], [a], [b], 1, max_norm=1.0)
+        genre.clip_adam_step_([q], [g], [c], [d], 1, max_norm=1.0)
+        assert torch.equal(a, c) and torch.equal(b, d)
+        assert p[3].item() == math.inf and p[36].item() == -math.inf and math.isnan(p[20].item())
+        p[3], p[36], p[20] = q[3], q[36], q[20]
+        assert torch.equal(p, q)
+
+
 def test_refusals(genre, dev):
     t, s = [torch.zeros(4, device=dev)], [torch.zeros(4, device=dev)]
     for bad in (lambda: genre.grad_norm(t, 1.0), lambda: genre.grad_norm([torch.zeros(3)]), lambda: genre.grad_norm([t[0].double()]),
