@@ -9,7 +9,8 @@ class ClipAdam(torch.optim.Adam):
     torch.nn.utils.clip_grad_norm_(all parameters, max_grad_norm) had run before every step, in a few launches for the whole
     network: the gradients are read twice and never written.  The norm that a step found is left in `grad_norm`, on the GPU.
 
-    Not for capture in a HIP graph: a replay would repeat the step that was captured, its count with it.  The moments are fp32 whatever the weights' type.  Parameters without a gradient are passed over, as they are there."""
+    Not for capture in a HIP graph: a replay would repeat the step that was captured, its count with it.  The moments are fp32
+    whatever the weights' type.  Parameters without a gradient are passed over, as they are there."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0, max_grad_norm=None, decoupled_weight_decay=False):
         if max_grad_norm is not None and not max_grad_norm >= 0:
@@ -18,10 +19,13 @@ class ClipAdam(torch.optim.Adam):
         self.max_grad_norm = max_grad_norm
         self.grad_norm = None
 
+    def __getstate__(self):                                            # (copies and pickles)
+        return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, grad_norm=self.grad_norm)
+
     def _moments(self, p):
         st = self.state[p]
         if not st:
-            st["step"] = torch.tensor(0.0)
+            st["step"] = torch.tensor(0.0, dtype=torch.float32, device="cpu")
             st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
             st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
         elif st["exp_avg"].dtype != torch.float32:                     # a loaded state takes the weights' type
@@ -68,7 +72,7 @@ class ClipAdam(torch.optim.Adam):
             clip_adam_step_(params, grads, [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states], count + 1, lr=float(group["lr"]),
                             betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                             decoupled=group.get("decoupled_weight_decay", False), factor=factor)
-            now = torch.tensor(float(count + 1))
+            now = torch.tensor(float(count + 1), dtype=torch.float32, device="cpu")
             for s in states:
                 s["step"] = now
         return loss

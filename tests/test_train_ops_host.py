@@ -170,3 +170,12 @@ def test_the_plain_optimiser_stays_the_default(genre):
     assert type(adam(ps, 1e-3, (0.5, 0.9))) is torch.optim.Adam
     clip = adam(ps, 1e-3, (0.5, 0.9), 2.0)
     assert type(clip) is genre.ClipAdam and clip.max_grad_norm == 2.0 and clip.param_groups[0]["betas"] == (0.5, 0.9)
+
+
+def test_copies_of_an_optimiser_keep_its_bound(genre):
+    import copy
+    import pickle
+    opt = genre.ClipAdam([torch.nn.Parameter(torch.zeros(3))], lr=0.5, max_grad_norm=2.0)
+    for again in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert again.max_grad_norm == 2.0 and again.grad_norm is None and again.param_groups[0]["lr"] == 0.5
+        again.step()
