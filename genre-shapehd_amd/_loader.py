@@ -320,6 +320,8 @@ class _TrainingLib:
     and ctypes would take longer than the kernels.  Loaded at the first use and bound to this module's library."""
 
     def __getattr__(self, name):
+        if name.startswith("__"):                                          # (what copy or inspect ask of any object)
+            raise AttributeError(name)
         if not os.path.exists(BINDING_PATH):
             raise ImportError("genre-shapehd_amd: %s is not built. Run `make -C genre-shapehd_amd/csrc`" % BINDING_PATH)
         spec = importlib.util.spec_from_file_location("genre_torch", BINDING_PATH)

@@ -209,8 +209,8 @@ __global__ __launch_bounds__(kThreads) void adam_kernel(const Table<4> t, const 
 
 // ---- host -------------------------------------------------------------------------------------------------------
 // A launch's values per workgroup: some `workgroups` of them for what its table holds, 4 accesses of a thread at least, 128 at
-// most.  The norm takes 2048, the number that the chip holds at once (1024 / 1536 / 2048 / 3072 / 4096: 45.3 / 42.0 / 42.8 / 47.7 /
-// 44.1 us for the refiner's 214 MB, a last round half empty costing most); the Adam step, whose workgroups move seven streams, four
+// most.  The norm takes 2048, the number that the chip holds at once (1024 / 1536 / 2048 / 4096: 45.3 / 42.0 / 42.8 / 44.1 us for
+// the refiner's 214 MB); the Adam step, whose workgroups move seven streams, four
 // times that (2048 / 4096 / 6144 / 8192: 633 / 619 / 617 / 603 us for 93 million weights).  By the list's total instead, the shorter
 // tables of a long list did not fill the chip (98 us against 85 for the joint model's norm).
 constexpr int kNormWorkgroups = 2048, kAdamWorkgroups = 8192;

@@ -16,8 +16,8 @@
 // the passes cost 5 to 9 us.  What is read twice is the price: an image's group does not fit a CU, and a wait of workgroups for one
 // another inside a launch would need all of them resident.  Bound: HBM, at what a copy reaches (4.9 to 5.3 TB/s) or above it,
 // where the second pass, which starts where the first ended, still finds x in the 256 MB cache.  Measured:
-//   4 x 20 x 64^3 fp32 channels last, leaky ReLU: forward 17 + 31 us (84 MB read, 84 MB read + 86 written), backward 29 + 44 us
-//   8 x 32 x 64^3 bf16 channels first, ReLU:      forward 23 + 42 us (134 MB,       134 + 134),            backward 41 + 61 us
+//   4 x 20 x 64^3 fp32 channels last, leaky ReLU: forward 17 + 30 us (84 MB read, 84 MB read + 86 written), backward 28 + 42 us
+//   8 x 32 x 64^3 bf16 channels first, ReLU:      forward 22 + 42 us (134 MB,       134 + 134),            backward 41 + 61 us
 // y and dx are stored past the caches: a launch's end waits for what it left dirty in the L2s (58.7 -> 47.4 us and 88.8 -> 73.4).
 #include "group_norm.hpp"
 
@@ -63,8 +63,9 @@ struct Between {
 template <class T>
 __device__ __forceinline__ Stat stat_of(const Map &x, const Shape &sh, int n, int g, double s, double q)
 {
+    // (equal values: the mean is theirs, exactly; a NaN stays one)
     const double d = s / sh.m, var = fma(-d, d, q / sh.m);
-    return {first_value<T>(x, sh, n, g) + d, 1. / sqrt((var < 0 ? 0. : var) + sh.eps), 0, 0};      // (equal values: the mean is theirs, exactly; a NaN stays one)
+    return {first_value<T>(x, sh, n, g) + d, 1. / sqrt((var < 0 ? 0. : var) + sh.eps), 0, 0};
 }
 __device__ __forceinline__ void keep_stat(const Shape &sh, double *stats, int at, const Stat &t)
 {
@@ -299,7 +300,8 @@ __global__ __launch_bounds__(columns_of(V)) void last_value_kernel(Map x, Map dy
         if (c < sh.C) channel_grads(sh, bt.chunks, bt.chan, bt.stats, c, bt.dw, bt.dwt, bt.db, bt.dbt);
         return;
     }
-    const Where at = where(bt.blocks - 1 - blockIdx.x, cut.tiles, cut.chunks);           // from the end: what the first pass read last is still in the cache
+    // from the end: what the first pass read last is still in the cache
+    const Where at = where(bt.blocks - 1 - blockIdx.x, cut.tiles, cut.chunks);
     if (bt.joined) {
         const int each = blockDim.x / sh.G, g = threadIdx.x % sh.G, lane = threadIdx.x / sh.G;
         double2 t = make_double2(0, 0);
@@ -493,7 +495,11 @@ int check_param(const char *op, const char *what, const genre_tensor *t, int64_t
     return 1;
 }
 
-inline bool channels_last(const genre_tensor *t) { return t->size[1] == 1 ? t->stride[2] != 1 && t->size[2] != 1 : t->stride[1] == 1 && (t->size[2] == 1 || t->stride[2] != 1); }
+inline bool channels_last(const genre_tensor *t)
+{
+    if (t->size[1] == 1) return t->stride[2] != 1 && t->size[2] != 1;
+    return t->stride[1] == 1 && (t->size[2] == 1 || t->stride[2] != 1);
+}
 inline bool channels_first(const genre_tensor *t) { return t->size[2] == 1 || t->stride[2] == 1; }
 inline bool gapless(const genre_tensor *t) { return t->size[2] == 1 || t->stride[2] == t->size[1]; }
 inline Map map_of(const genre_tensor *t) { return {t->data, t->stride[0], t->stride[1], t->size[2] == 1 ? t->size[1] : t->stride[2]}; }

@@ -28,8 +28,8 @@ __device__ __forceinline__ void store(typename T::raw *p, const float (&v)[V])
     else *(W *)p = t;
 }
 
-// Loads and stores of V values need no more than their type's own alignment (gfx950 moves 16 bytes at any address).
-// V values as they lie in memory: a thread keeps these, two 16-bit values to a register, and converts them in each pass
+// V values as they lie in memory: a thread keeps these, two 16-bit values to a register, and converts them in each pass.  Loads and
+// stores need no more than their type's own alignment (gfx950 moves 16 bytes at any address).
 template <class T, int V>
 struct Kept {
     static constexpr int kWords = (V * sizeof(typename T::raw) + 3) / 4;
@@ -124,7 +124,6 @@ __device__ __forceinline__ void block_sum2(double &a, double &b, double *lds)
     }
 }
 
-
 struct Params { const void *w, *b; int wt, bt; };
 struct Grads { Map dx; void *dw, *db; int dwt, dbt; };
 
@@ -133,7 +132,6 @@ __device__ __forceinline__ double first_value(const Map &x, const Shape &sh, int
 {
     return (double)(float)((const typename T::raw *)x.p)[n * x.sn + (int64_t)g * sh.cg * x.sc];
 }
-
 
 // The chunks' sums lie in the workspace as double2 [image][chunk][channel] of dz and dz (x - mean) (one chunk: an image's).
 // dw and db of one channel from them, by one wave: in this order whatever order the workgroups that left them ended in.

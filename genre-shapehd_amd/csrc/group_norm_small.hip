@@ -1,7 +1,9 @@
 // group_norm_small.hip -- group normalisation where one workgroup holds an image's group in its registers.
 //
-// A map whose groups hold up to 16384 values (backward: 8192 channels last, 4096 first) takes one launch, reads x (and dy) once, and needs no scratch.  A group is `rows` runs of `cols` accesses of V values: channels last, a run is one position's cg channels and every
-// thread keeps one column; channels first, a run is one channel's positions, shared by a team of 2^k threads.
+// A map whose groups hold up to 16384 values (backward: 8192 channels last, 4096 first) takes one launch (backward of several images:
+// and one that adds up their dw and db) and reads x (and dy) once.  A group is `rows` runs of `cols` accesses of V values: channels
+// last, a run is one position's cg channels and every thread keeps one column; channels first, a run is one channel's positions,
+// shared by a team of 2^k threads.
 //
 // Bound: latency -- one load's way to memory and back, two sums over a workgroup, the stores: 3.5 us for 640 channels of one
 // position, 5.8 for 10240 values a group, against 8 to 10 us in the two passes of group_norm.hip.  With 64 values a thread instead of
@@ -17,8 +19,9 @@ using namespace gn;
 constexpr int kThreads = 1024, kBackwardThreads = 512, kValues = 16;
 
 struct Small {
-    int rows, cols, team, deep, turns, subs;                               // threads of a run, runs at once, accesses of a thread and run, waves of a team
-    int64_t gsx, gsd, gso, psx, psd, pso;                             // a run's stride and a group's in x, dy, out (elements)
+    int rows, cols;
+    int team, deep, turns, subs;                                           // threads of a run, runs at once, accesses of a thread and run, waves of a team
+    int64_t gsx, gsd, gso, psx, psd, pso;                                  // a group's stride and a run's in x, dy, out (elements)
 };
 
 // a run-time activation -- a kernel for each would be four times as many -- chosen once around a loop over the values

@@ -65,7 +65,8 @@ class WGANGP:
     def __init__(self, net_g=None, net_d=None, nz=200, lr=1e-4, betas=(0.5, 0.9), lam=10.0, norm=1.0, d_iter=1,
                  generator=None, gen_norm="batch", clip_grad=None):
         """gen_norm: the default generator's normalisation, "batch" or "group".  clip_grad: bound on the norm of each network's
-        gradients (ClipAdam; None: not bounded, as in the reference).  generator: optional CPU torch.Generator -- latent codes and the interpolation weights of the penalty are then
+        gradients (ClipAdam; None: not bounded, as in the reference).
+        generator: optional CPU torch.Generator -- latent codes and the interpolation weights of the penalty are then
         drawn on the host from it and copied to the device (a run is reproducible across devices); default: drawn on
         the device, as the reference does (wgangp.py:98,134)"""
         self.net_g = net_g if net_g is not None else VoxelGenerator(nz, norm=gen_norm)

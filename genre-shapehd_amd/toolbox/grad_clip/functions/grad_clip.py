@@ -31,7 +31,8 @@ def _bound(op, max_norm):
 
 def grad_norm(tensors, norm_type=2.0):
     """norm of the vector of all the tensors' values (2: Euclidean, fp64 sums; inf: the largest magnitude) as an fp32 tensor of no
-    dimensions on their GPU.  NaN where a value is NaN.  It carries no gradient.  An empty list has the norm 0 (on the CPU, as nothing names a GPU)."""
+    dimensions on their GPU.  NaN where a value is NaN.  It carries no gradient.  An empty list
+    has the norm 0 (on the CPU, as nothing names a GPU)."""
     kind, tensors = _kind("grad_norm", norm_type), _list(tensors)
     return _native.grad_norm(tensors, math.inf, kind)[0] if tensors else torch.tensor(0.0)
 
@@ -54,8 +55,9 @@ def clip_adam_step_(params, grads, exp_avgs, exp_avg_sqs, step, *, lr=1e-3, beta
                     max_norm=None, norm_type=2.0, factor=None):
     """one Adam step on `params` in place, `exp_avgs` and `exp_avg_sqs` with them, as if clip_grads_(grads, max_norm, norm_type) had
     run before -- without writing the gradients.  step counts from 1 (a captured call replays with the one it was given).
-    weight_decay is added to the gradient, or (decoupled) shrinks the weights by lr * weight_decay.  params[i] and grads[i] have one type and layout, the states are fp32 in that layout;
-    tensors that share memory are refused (gradients may, with each other).  Returns the norm of the gradients before the clip (None without max_norm).
+    weight_decay is added to the gradient, or (decoupled) shrinks the weights by lr * weight_decay.  params[i] and grads[i]
+    have one type and layout, the states are fp32 in that layout; tensors that share memory are refused (gradients may, with each
+    other).  Returns the norm of the gradients before the clip (None without max_norm).
     factor (instead of max_norm): one fp32 value on the same GPU that the gradients are multiplied by -- for weights that are
     stepped in several calls under one clip."""
     kind = _kind("clip_adam_step_", norm_type)

@@ -456,9 +456,10 @@ int genre_render_bm_backward(const genre_tensor *grad_out, const genre_tensor *g
  *   forward:  y = act((x - mean) / sqrt(var + eps) * weight + bias), mean and biased variance of each image and group;
  *             stats fp64 [2,N,groups] receives mean and 1 / sqrt(var + eps)
  *   backward: from x, dy and the forward's stats; dx (NULL: not wanted), dw, db
- * ws: fp64 scratch of at least genre_group_norm_workspace(x, groups, backward) values (-1: refused; 0: may be NULL), undefined before and after;
- * two calls that may run at once need two.  Sums and statistics are fp64 and added in a fixed order: equal inputs, equal bits.
- * The derivative of (leaky) ReLU at 0 is that of the negative side.  N or S of zero: nothing but dw = db = 0 is written. */
+ * ws: fp64 scratch of at least genre_group_norm_workspace(x, groups, backward) values (-1: refused; 0: may be NULL), undefined
+ * before and after; two calls that may run at once need two.  Sums and statistics are fp64 and added in a fixed order: equal inputs, equal bits.
+ * No output may share memory with an input or another output.  The derivative of (leaky) ReLU at 0 is that of the negative side;
+ * a ReLU that is off passes nothing on, whatever dy holds there.  N or S of zero: nothing but dw = db = 0 is written. */
 int64_t genre_group_norm_workspace(const genre_tensor *x, int groups, int backward);
 
 int genre_group_norm_forward(const genre_tensor *x, const genre_tensor *y, const genre_tensor *weight, const genre_tensor *bias,
@@ -477,8 +478,8 @@ int genre_group_norm_backward(const genre_tensor *x, const genre_tensor *dy, con
  *     0: the largest magnitude (NaN if one is) -- and the factor min(1, max_norm / (norm + 1e-6)) (NaN stays NaN; 1 for
  *     max_norm = infinity).  ws: fp64 scratch of at least genre_grad_workspace(numels, n) values.
  *   genre_grad_scale: every value times factor[0] (fp32, on the device), rounded to its type; 1 leaves the memory untouched
- *   genre_adam_step: with g' = g factor[0] + weight_decay p (factor NULL: 1; weight_decay 0: g factor[0], whatever p; decoupled != 0: p is scaled by 1 - lr weight_decay
- *     instead),  m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2,
+ *   genre_adam_step: with g' = g factor[0] + weight_decay p (factor NULL: 1; weight_decay 0: g factor[0], whatever p;
+ *     decoupled != 0: p is scaled by 1 - lr weight_decay instead),  m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2,
  *     p -= lr / (1 - beta1^step) m / (sqrt(v / (1 - beta2^step)) + eps);  p and g of dtypes[i], m and v fp32; g is not written. */
 int64_t genre_grad_workspace(const int64_t *numels, int n);
 
