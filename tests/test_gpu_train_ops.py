@@ -233,6 +233,79 @@ def test_what_autograd_guards(genre, dev):
         y.sum().backward()
 
 
+def test_broadcast_inputs(genre, dev):
+    """one image for a whole batch, one weight for all channels: their gradients are the sums of what each copy gets, which are those
+    of the copies laid out (bits; the sums over four and eight fp32 terms are torch's, (n - 1) u of the terms' magnitudes apart at most)"""
+    for shape in ((1, 8, 5, 9), (1, 8, 60, 71)):
+        x, w, b, dy = torch.randn(shape, device=dev), torch.randn(1, device=dev), torch.randn(8, device=dev), torch.randn(4, *shape[1:], device=dev)
+        one = [t.clone().requires_grad_(True) for t in (x, w, b)]
+        y = genre.group_norm_act(one[0].expand(4, -1, -1, -1), 2, one[1].expand(8), one[2], act="silu")
+        dx, dw, db = torch.autograd.grad(y, one, dy)
+        all_ = [t.clone().requires_grad_(True) for t in (x.repeat(4, 1, 1, 1), w.repeat(8), b)]
+        z = genre.group_norm_act(all_[0], 2, all_[1], all_[2], act="silu")
+        ex, ew, eb = torch.autograd.grad(z, all_, dy)
+        assert torch.equal(y, z) and torch.equal(db, eb)
+        for got, each in ((dx, ex), (dw, ew.unsqueeze(1))):
+            off = (got.double() - each.double().sum(0, keepdim=True).view(got.shape)).abs()
+            assert bool((off <= 8 * U * each.double().abs().sum(0, keepdim=True).view(got.shape)).all())
+
+
+def test_two_passes_captured_and_replayed(genre, dev):
+    """maps that take scratch memory: two graphs with an eager call between their replays, each result the eager one's bits"""
+    graphs = []
+    for fmt, shape in ((torch.channels_last_3d, (2, 40, 20, 21, 22)), (torch.contiguous_format, (2, 24, 30, 31, 9))):
+        x, dy = (torch.randn(shape, device=dev).contiguous(memory_format=fmt) for _ in range(2))
+        leaves = [t.clone().requires_grad_(True) for t in (x, torch.randn(shape[1], device=dev), torch.randn(shape[1], device=dev))]
+        step = lambda leaves=leaves, dy=dy: [(y := genre.group_norm_act(leaves[0], 8, *leaves[1:], act="relu")).detach(), *torch.autograd.grad(y, leaves, dy)]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        graphs.append((graph, leaves, dy, step, got))
+    for turn in range(3):
+        wants = []
+        for graph, leaves, dy, step, got in graphs:
+            with torch.no_grad():
+                leaves[0].normal_()
+                dy.normal_()
+            wants.append([t.clone() for t in step()])
+        for graph, *_ in graphs:
+            graph.replay()
+            graphs[0][3]()
+        torch.cuda.synchronize()
+        for (*_, got), want in zip(graphs, wants):
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_threads_at_once(genre, dev):
+    """each on a stream of its own, as data-parallel programs call: the bits of one after the other"""
+    import threading
+    x = torch.randn(2, 40, 20, 21, 22, device=dev)
+    lists = [[torch.randn(s, device=dev) for s in ((5000,), (33, 7), (1,))] for _ in range(2)]
+    want = [(genre.group_norm_act(x, 8, act="silu"), genre.grad_norm(ts)) for ts in lists]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                y, norm = genre.group_norm_act(x, 8, act="silu"), genre.grad_norm(lists[i])
+            torch.cuda.current_stream().synchronize()
+        got[i] = (y, norm)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for g, w in zip(got, want):
+        assert torch.equal(g[0], w[0]) and torch.equal(g[1], w[1])
+
+
 def test_views_of_negatives(genre, dev):
     """torch's lazy negation (of a conjugate's imaginary part) is a flag on the tensor, not in its memory"""
     x, dy, w = (torch.randn(s, device=dev) for s in ((2, 8, 4, 4), (2, 8, 4, 4), (8,)))
