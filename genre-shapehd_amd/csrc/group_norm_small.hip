@@ -142,10 +142,11 @@ __global__ __launch_bounds__(kThreads) void small_forward_kernel(Map x, Map y, S
     });
 }
 
-// chan: the sums of dz and dz (x - mean) by image and channel (more than one image: added up behind this), or dw and db themselves
+// chan: the sums of dz and dz (x - mean) by image and channel (more than one image: added up behind this), or dw and db themselves,
+// whose types need not be those of weight and bias
 template <class T, int V, bool LAST>
 __global__ __launch_bounds__(kBackwardThreads) void small_backward_kernel(Map x, Map dy, Map dx, Shape sh, Small m, const double *stats, const void *w, const void *b, int wt,
-                                                             int bt, double2 *chan, void *dw, void *db)
+                                                             int bt, double2 *chan, void *dw, void *db, int dwt, int dbt)
 {
     using R = typename T::raw;
     constexpr int K = kValues / V;
@@ -232,8 +233,8 @@ __global__ __launch_bounds__(kBackwardThreads) void small_backward_kernel(Map x,
         }
         if (chan) chan[(int64_t)n * sh.C + g * cg + c] = a;
         a.y *= r;
-        if (db) store_param(db, bt, g * cg + c, a.x);
-        if (dw) store_param(dw, wt, g * cg + c, a.y);
+        if (db) store_param(db, dbt, g * cg + c, a.x);
+        if (dw) store_param(dw, dwt, g * cg + c, a.y);
         m1 = fma(coef[2 * cg + c], a.x, m1);
         m2 = fma(coef[2 * cg + c], a.y, m2);
     }
@@ -332,7 +333,8 @@ int backward_as(const Shape &sh, const SmallCall &k, const Map &x, const Map &dy
     const bool one = sh.N == 1;
     const size_t lds = sizeof(double) * (3 * sh.cg + (sh.cg & 1)) + sizeof(double2) * (LAST ? V * k.threads : sh.cg * k.m.subs);
     double2 *chan = !one && (g.dw || g.db) ? (double2 *)ws : nullptr;
-    small_backward_kernel<T, V, LAST><<<sh.N * sh.G, k.threads, lds, st>>>(x, dy, g.dx, sh, k.m, stats, p.w, p.b, p.wt, p.bt, chan, one ? g.dw : nullptr, one ? g.db : nullptr);
+    small_backward_kernel<T, V, LAST><<<sh.N * sh.G, k.threads, lds, st>>>(x, dy, g.dx, sh, k.m, stats, p.w, p.b, p.wt, p.bt, chan, one ? g.dw : nullptr, one ? g.db : nullptr,
+                                                                              g.dwt, g.dbt);
     GENRE_LAUNCH_CHECK("group norm backward");
     if (chan) {
         channel_grads_kernel<<<ceil_div(sh.C, 4), 256, 0, st>>>(sh, 1, chan, stats, g.dw, g.dwt, g.db, g.dbt);
