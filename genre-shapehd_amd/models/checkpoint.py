@@ -6,6 +6,8 @@ Reloading an optimizer keeps the CURRENT training hyper-parameters (learning rat
 moments and step counts from the file, as the reference does when a run is resumed with new options."""
 import torch
 
+from ..optim import own_steps
+
 
 def save_state_dict(path, nets, optimizers=None, **additional_values):
     state = {"nets": [n.state_dict() for n in nets]}
@@ -16,6 +18,8 @@ def save_state_dict(path, nets, optimizers=None, **additional_values):
 
 
 def optimizer_load_state_dict(optimizer, state, keep_training_params=False):
+    if "state" in state:
+        state = dict(state, state=own_steps(state["state"]))              # (files from before ClipAdam.state_dict held shared ones)
     if keep_training_params:
         current = optimizer.state_dict()["param_groups"]
         assert len(current) == len(state["param_groups"])

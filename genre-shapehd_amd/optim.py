@@ -4,6 +4,12 @@ import torch
 from .toolbox.grad_clip.functions.grad_clip import _native, clip_adam_step_
 
 
+def own_steps(states):
+    """the `state` of an optimiser's state_dict with a `step` of its own in every entry (torch.optim.Adam counts in place, and loads
+    and saves keep tensors that are shared)"""
+    return {k: dict(st, step=st["step"].clone()) if isinstance(st, dict) and torch.is_tensor(st.get("step")) else st for k, st in states.items()}
+
+
 class ClipAdam(torch.optim.Adam):
     """torch.optim.Adam (state_dicts go from one to the other) on GPU tensors, as if
     torch.nn.utils.clip_grad_norm_(all parameters, max_grad_norm) had run before every step, in a few launches for the whole
@@ -21,6 +27,11 @@ class ClipAdam(torch.optim.Adam):
 
     def __getstate__(self):                                            # (copies and pickles)
         return dict(super().__getstate__(), max_grad_norm=self.max_grad_norm, grad_norm=self.grad_norm)
+
+    def state_dict(self):
+        """torch.optim.Adam's (parameters that are stepped together share one `step` here, which stays inside)"""
+        out = super().state_dict()
+        return dict(out, state=own_steps(out["state"]))
 
     def _moments(self, p):
         st = self.state[p]
