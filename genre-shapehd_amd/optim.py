@@ -33,14 +33,32 @@ class ClipAdam(torch.optim.Adam):
         out = super().state_dict()
         return dict(out, state=own_steps(out["state"]))
 
+    def load_state_dict(self, state_dict):
+        """torch.optim.Adam's too.  torch casts what it loads to the weights' type, in which a resumed run would not be the one that
+        was saved (an fp16 second moment is zero below 3e-8): the moments are taken from the given state, in fp32"""
+        given = []                                                     # as the hooks leave it
+        hooks = [self.register_load_state_dict_pre_hook(lambda _, sd: given.append(sd)),
+                 self.register_load_state_dict_post_hook(lambda _: self._keep_moments(given[-1]), prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _keep_moments(self, given):
+        keys = [k for group in given["param_groups"] for k in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for key, p in zip(keys, params):
+            for name in ("exp_avg", "exp_avg_sq"):
+                if name in given["state"].get(key, {}) and self.state[p][name].dtype != torch.float32:
+                    self.state[p][name] = given["state"][key][name].detach().to(p.device, torch.float32, copy=True)
+
     def _moments(self, p):
         st = self.state[p]
         if not st:
             st["step"] = torch.tensor(0.0, dtype=torch.float32, device="cpu")
             st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
             st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
-        elif st["exp_avg"].dtype != torch.float32:                     # a loaded state takes the weights' type
-            st["exp_avg"], st["exp_avg_sq"] = st["exp_avg"].float(), st["exp_avg_sq"].float()
         return st
 
     @torch.no_grad()

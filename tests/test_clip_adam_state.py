@@ -95,3 +95,65 @@ def test_files_with_a_shared_count_load_as_well(genre, foreach, tmp_path):
     _grads(params, 1)
     again.step()
     assert [float(again.state[p]["step"]) for p in params] == [5.0] * 4
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16), ids=("fp32", "bf16", "fp16"))
+def test_a_resumed_run_is_the_one_that_was_saved(optim, dtype):
+    """bits, with gradients so small that an fp16 second moment would be zero (1e-4 squared), through a file, a copy and a pickle"""
+    import pickle
+    ps = _weights(dtype)
+    opt = optim.ClipAdam(ps, lr=1e-2, betas=(0.5, 0.9))
+    _grads(ps, 0, 1e-4)
+    opt.step()
+    runs = [(ps, opt)]
+    for way in (_through_a_file, copy.deepcopy):
+        qs = [torch.nn.Parameter(p.detach().clone()) for p in ps]
+        again = optim.ClipAdam(qs, lr=1e-2, betas=(0.5, 0.9))
+        again.load_state_dict(way(opt.state_dict()))
+        runs.append((qs, again))
+    whole = pickle.loads(pickle.dumps(opt))
+    runs.append((whole.param_groups[0]["params"], whole))
+    for step in (2, 3):
+        for qs, o in runs:
+            _grads(qs, step, 1e-4)
+            o.step()
+    for qs, o in runs[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+        for p, q in zip(ps, qs):
+            assert all(torch.equal(opt.state[p][k], o.state[q][k]) and o.state[q][k].dtype == torch.float32 for k in ("step", "exp_avg", "exp_avg_sq"))
+
+
+def test_loaded_moments_are_the_ones_that_the_hooks_leave(optim):
+    """and no memory of the state that was loaded"""
+    ps = _weights(torch.float16)
+    opt = optim.ClipAdam(ps, lr=1e-2)
+    _grads(ps, 0)
+    opt.step()
+    again = optim.ClipAdam([torch.nn.Parameter(p.detach().clone()) for p in ps], lr=1e-2)
+    half = lambda o, sd: dict(sd, state={k: dict(st, exp_avg=st["exp_avg"] / 2) for k, st in sd["state"].items()})
+    again.register_load_state_dict_pre_hook(half)
+    sd = opt.state_dict()
+    again.load_state_dict(sd)
+    for p, q in zip(ps, again.param_groups[0]["params"]):
+        assert torch.equal(again.state[q]["exp_avg"], opt.state[p]["exp_avg"] / 2)
+        again.state[q]["exp_avg_sq"].zero_()
+        assert bool((opt.state[p]["exp_avg_sq"] > 0).all())
+    again.load_state_dict(sd)                                             # (no hook of the first load is left)
+    again.load_state_dict(optim.ClipAdam(ps).state_dict())                # no state at all
+    assert not again.state
+
+
+def test_a_state_that_half_precision_adam_wrote(optim):
+    """its moments, which are half precision there"""
+    ps = _weights(torch.bfloat16)
+    adam = torch.optim.Adam(ps, lr=1e-2)
+    _grads(ps, 0)
+    adam.step()
+    opt = optim.ClipAdam([torch.nn.Parameter(p.detach().clone()) for p in ps], lr=1e-2)
+    opt.load_state_dict(adam.state_dict())
+    qs = opt.param_groups[0]["params"]
+    for p, q in zip(ps, qs):
+        assert all(opt.state[q][k].dtype == torch.float32 and torch.equal(opt.state[q][k], adam.state[p][k].float()) for k in ("exp_avg", "exp_avg_sq"))
+    _grads(qs, 1)
+    opt.step()
+    assert {float(opt.state[q]["step"]) for q in qs} == {2.0}
