@@ -17,8 +17,6 @@ import math
 import torch
 from torch import nn
 
-from ..toolbox.group_norm.modules.group_norm import GroupNormAct
-
 from .resnet import resnet18
 from .thin_conv import ThinConv3d, ThinConvTranspose3d
 
@@ -37,11 +35,21 @@ def _down3(cin, cout, bias):               # /2
     return ThinConv3d(cin, cout, 4, 2, 1, bias=bias)
 
 
+def _group_norm(*args, **kwargs):
+    # imported at its first use: this file serves `networks` as a top-level package too, beside `toolbox`, and needs no native
+    # library unless a network asks for this operator
+    if "." in __package__:
+        from ..toolbox.group_norm.modules.group_norm import GroupNormAct
+    else:
+        from toolbox.group_norm.modules.group_norm import GroupNormAct
+    return GroupNormAct(*args, **kwargs)
+
+
 def _norm_act3(c, norm, act):
     """[normalisation, activation] of c channels; "group": one operator does both, and an empty module keeps the indices"""
     if norm == "group":
         name, slope = ("relu", 0.0) if isinstance(act, nn.ReLU) else ("leaky_relu", act.negative_slope)
-        return [GroupNormAct(math.gcd(c, 8), c, act=name, slope=slope), nn.Identity()]
+        return [_group_norm(math.gcd(c, 8), c, act=name, slope=slope), nn.Identity()]
     if norm != "batch":
         raise ValueError("norm must be 'batch' or 'group', got %r" % (norm,))
     return [nn.BatchNorm3d(c), act]
