@@ -483,8 +483,8 @@ int check_map(const char *op, const char *what, const genre_tensor *t, const gen
     GENRE_REQUIRE(t && t->ndim == 3 && is_map_type(t->dtype), "%s: %s must be a [N,C,S] tensor of fp32, bf16 or fp16", op, what);
     GENRE_REQUIRE(same_shape(t, like), "%s: %s must have x's shape", op, what);
     GENRE_REQUIRE(t->dtype == like->dtype, "%s: %s must have x's dtype", op, what);
+    for (int i = 0; i < 3; i++) GENRE_REQUIRE(t->size[i] >= 0 && t->stride[i] >= 0, "%s: %s has a negative size or stride", op, what);
     GENRE_REQUIRE(t->data || numel(t) == 0, "%s: %s is NULL", op, what);
-    for (int i = 0; i < 3; i++) GENRE_REQUIRE(t->stride[i] >= 0, "%s: %s has a negative stride", op, what);
     return 1;
 }
 int check_param(const char *op, const char *what, const genre_tensor *t, int64_t C)
@@ -607,6 +607,7 @@ int plan(const char *op, const genre_tensor *x, const genre_tensor *const *other
     const int64_t N = x->size[0], C = x->size[1], S = x->size[2];
     GENRE_REQUIRE(groups > 0 && C > 0 && C % groups == 0, "%s: %lld channels do not split into %d groups", op, (long long)C, groups);
     GENRE_REQUIRE(N * C < (1 << 30), "%s: N*C must be below 2^30", op);
+    GENRE_REQUIRE(N == 0 || S < ((int64_t)1 << 60) / (N * C), "%s: a map of 2^60 values or more", op);
     bool last = channels_last(x), first = channels_first(x), dense = gapless(x);
     for (int i = 0; i < n_others; i++) {
         last = last && channels_last(others[i]);

@@ -1,0 +1,28 @@
+"""The C entries of the training-step ops without a GPU: sizes that no tensor has are refused, and end no process."""
+import ctypes as C
+
+import pytest
+
+from test_train_ops_host import F64, desc, lib  # noqa: F401
+
+I64 = 1 << 62
+
+
+def entries(L, lib, x, groups=2, act=1):
+    """{name: the refusal of one map by every entry that takes one}"""
+    big, stats = desc(L, (1 << 20,), dtype=F64), desc(L, (2, 2, 2), dtype=F64)
+    g, a, s = C.c_int(groups), C.c_int(act), C.c_float(0.1)
+    calls = {"workspace": lambda: lib.genre_group_norm_workspace(x, g, C.c_int(0)) + 1, "backward workspace": lambda: lib.genre_group_norm_workspace(x, g, C.c_int(1)) + 1,
+             "forward": lambda: lib.genre_group_norm_forward(x, x, None, None, stats, big, g, C.c_double(1e-5), a, s, None),
+             "backward": lambda: lib.genre_group_norm_backward(x, x, None, None, stats, x, None, None, big, g, a, s, None)}
+    return {name: (call(), lib.genre_last_error()) for name, call in calls.items()}
+
+
+@pytest.mark.parametrize("shape,stride,word", (
+    ((2, 6, -5), (30, 5, 1), b"negative size"), ((-2, 6, 50000), (300000, 50000, 1), b"negative size"), ((-2, 6, -50000), (300000, 50000, 1), b"negative size"),
+    ((2, -6, 50), (300, 50, 1), b"negative size"), ((2, 6, 50), (300, -50, 1), b"negative size or stride"),
+    ((2, 6, I64), (0, I64, 1), b"2^60"), ((2, 6, I64 // 4 + 3), (0, I64, 1), b"2^60"), ((1, 1 << 20, 1 << 44), (0, 1 << 44, 1), b"2^60")))
+def test_sizes_that_no_map_has(lib, shape, stride, word):  # noqa: F811
+    L, lib = lib
+    for name, (rc, error) in entries(L, lib, desc(L, shape, stride=stride)).items():
+        assert rc == 0 and word in error, (name, error)
