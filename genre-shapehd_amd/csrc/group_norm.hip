@@ -476,6 +476,7 @@ __global__ __launch_bounds__(256) void group_sums_kernel(Shape sh, Between bt, c
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------
+inline int es_of(const genre_tensor *t) { return t->dtype == GENRE_F32 ? 4 : 2; }
 inline bool is_map_type(int32_t t) { return t == GENRE_F32 || t == GENRE_BF16 || t == GENRE_F16; }
 
 int check_map(const char *op, const char *what, const genre_tensor *t, const genre_tensor *like)
@@ -559,6 +560,7 @@ Run run_of(int N, int C, int64_t S, int v, int threads, int workgroups, int64_t 
 
 struct Call {
     Shape sh;
+    int small;                                                             // threads of a workgroup in the one-workgroup form (0: two passes)
     bool last, joined;
     int v, threads;
     Cut sums, values;                                                      // channels last
@@ -601,7 +603,10 @@ void cut_call(Call &c, int64_t N, int64_t C, int64_t S, int groups)
     }
 }
 
-int plan(const char *op, const genre_tensor *x, const genre_tensor *const *others, int n_others, int groups, Call &c)
+// a launch counts its threads in 32 bits
+inline bool launches(int64_t workgroups, int threads) { return workgroups * threads < ((int64_t)1 << 32); }
+
+int plan(const char *op, const genre_tensor *x, const genre_tensor *const *others, int n_others, int groups, bool backward, Call &c)
 {
     GENRE_REQUIRE(x->size[0] <= INT32_MAX && x->size[1] <= (1 << 24), "%s: too many images or channels", op);
     const int64_t N = x->size[0], C = x->size[1], S = x->size[2];
@@ -620,10 +625,12 @@ int plan(const char *op, const genre_tensor *x, const genre_tensor *const *other
     c.v = width_of(x, last, dense);
     if (N * S == 0) return 1;
     c.sh.m = (double)(C / groups) * (double)S;
+    c.small = small_threads(last, c.sh, es_of(x), backward);
     cut_call(c, N, C, S, groups);
-    GENRE_REQUIRE(c.sums_blocks() < INT32_MAX && c.value_blocks() + C < INT32_MAX && N * (int64_t)c.chunks() < INT32_MAX && N * groups < INT32_MAX / 2 &&
-                      c.chunks() * (C / groups) < INT32_MAX,
-                  "%s: the map is too large for one launch", op);
+    const bool fits = c.small ? launches(N * groups, c.small)
+                              : launches(c.sums_blocks(), c.threads) && launches(c.value_blocks() + C, c.threads) && (c.joined || launches(N * groups, 256)) &&
+                                    N * (int64_t)c.chunks() < INT32_MAX && c.chunks() * (C / groups) < INT32_MAX;
+    GENRE_REQUIRE(fits && N * groups < INT32_MAX / 2, "%s: the map is too large for one launch", op);
     return 1;
 }
 
@@ -727,7 +734,7 @@ int backward(const Call &c, const Map &x, const Map &dy, const Params &p, const 
 // scratch of a call whose maps all lie as `c` says
 int64_t needed(const Call &c, const genre_tensor *x, bool backward)
 {
-    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, backward)) return backward ? small_workspace(c.sh) : 0;
+    if (small_threads(c.last, c.sh, es_of(x), backward)) return backward ? small_workspace(c.sh) : 0;
     return workspace_of(c, backward);
 }
 
@@ -741,7 +748,7 @@ extern "C" int64_t genre_group_norm_workspace(const genre_tensor *x, int groups,
     const char *op = "group_norm_workspace";
     Call c{};
     if (!x) { fail("%s: x is NULL", op); return -1; }
-    if (!check_map(op, "x", x, x) || !plan(op, x, nullptr, 0, groups, c)) return -1;
+    if (!check_map(op, "x", x, x) || !plan(op, x, nullptr, 0, groups, backward != 0, c)) return -1;
     if (numel(x) == 0) return 0;
     int64_t need = needed(c, x, backward != 0);
     // the other maps may make another call of it: gaps in their rows narrow the columns, and with one position (which lies in both
@@ -769,7 +776,7 @@ extern "C" int genre_group_norm_forward(const genre_tensor *x, const genre_tenso
     GENRE_REQUIRE(act >= kActNone && act <= kActSilu, "%s: unknown activation %d", op, act);
     Call c{};
     const genre_tensor *const others[] = {y};
-    if (!plan(op, x, others, 1, groups, c)) return 0;
+    if (!plan(op, x, others, 1, groups, false, c)) return 0;
     if (!check_f64(op, "stats", stats, 2 * (int64_t)c.sh.N * groups)) return 0;
     if (numel(x) == 0) return 1;
     c.sh.act = act;
@@ -779,7 +786,7 @@ extern "C" int genre_group_norm_forward(const genre_tensor *x, const genre_tenso
     const Map mx = map_of(x), my = map_of(y);
     double *s = (double *)stats->data;
     hipStream_t st = (hipStream_t)stream;
-    if (small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, false)) return small_forward(c.last, x->dtype, c.sh, mx, my, p, s, st);
+    if (c.small) return small_forward(c.last, x->dtype, c.sh, mx, my, p, s, st);
     if (!check_f64(op, "ws", ws, workspace_of(c, false))) return 0;
     double *b = (double *)ws->data;
     if (x->dtype == GENRE_F32)
@@ -804,7 +811,7 @@ extern "C" int genre_group_norm_backward(const genre_tensor *x, const genre_tens
     GENRE_REQUIRE(act >= kActNone && act <= kActSilu, "%s: unknown activation %d", op, act);
     Call c{};
     const genre_tensor *const others[] = {dy, dx};
-    if (!plan(op, x, others, dx ? 2 : 1, groups, c)) return 0;
+    if (!plan(op, x, others, dx ? 2 : 1, groups, true, c)) return 0;
     if (!check_f64(op, "stats", stats, 2 * (int64_t)c.sh.N * groups)) return 0;
     hipStream_t st = (hipStream_t)stream;
     const Grads g = {dx ? map_of(dx) : Map{}, dw ? dw->data : nullptr, db ? db->data : nullptr, dw ? dw->dtype : 0, db ? db->dtype : 0};
@@ -822,10 +829,9 @@ extern "C" int genre_group_norm_backward(const genre_tensor *x, const genre_tens
     const Params p = {weight ? weight->data : nullptr, bias ? bias->data : nullptr, weight ? weight->dtype : 0, bias ? bias->dtype : 0};
     const Map mx = map_of(x), md = map_of(dy);
     const double *s = (const double *)stats->data;
-    const bool small = small_fits(c.last, c.sh, x->dtype == GENRE_F32 ? 4 : 2, true);
-    if (!check_f64(op, "ws", ws, small ? small_workspace(c.sh) : workspace_of(c, true))) return 0;
+    if (!check_f64(op, "ws", ws, c.small ? small_workspace(c.sh) : workspace_of(c, true))) return 0;
     double *b = ws ? (double *)ws->data : nullptr;
-    if (small) return small_backward(c.last, x->dtype, c.sh, mx, md, p, g, s, b, st);
+    if (c.small) return small_backward(c.last, x->dtype, c.sh, mx, md, p, g, s, b, st);
     if (x->dtype == GENRE_F32)
         return c.v == 4 ? backward<F32, 4>(c, mx, md, p, g, s, b, st) : c.v == 2 ? backward<F32, 2>(c, mx, md, p, g, s, b, st) : backward<F32, 1>(c, mx, md, p, g, s, b, st);
     if (x->dtype == GENRE_BF16)

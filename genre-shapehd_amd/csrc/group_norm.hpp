@@ -159,8 +159,8 @@ static __global__ __launch_bounds__(256) void channel_grads_kernel(Shape sh, int
 inline int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
 // ---- group_norm_small.hip ---------------------------------------------------------------------------------------
-// whether a call's groups are small enough for it
-bool small_fits(bool last, const Shape &sh, int es, bool backward);
+// the threads of its workgroups, one per image and group; 0: a call's groups are too large for it
+int small_threads(bool last, const Shape &sh, int es, bool backward);
 inline int64_t small_workspace(const Shape &sh) { return sh.N == 1 ? 0 : 2 * (int64_t)sh.N * sh.C; }       // fp64 values, backward
 int small_forward(bool last, int dtype, const Shape &sh, const Map &x, const Map &y, const Params &p, double *stats, hipStream_t st);
 int small_backward(bool last, int dtype, const Shape &sh, const Map &x, const Map &dy, const Params &p, const Grads &g, const double *stats, double *ws, hipStream_t st);

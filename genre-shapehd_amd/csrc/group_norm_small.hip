@@ -347,10 +347,10 @@ int backward_as(const Shape &sh, const SmallCall &k, const Map &x, const Map &dy
 
 namespace gn {
 
-bool small_fits(bool last, const Shape &sh, int es, bool backward)
+int small_threads(bool last, const Shape &sh, int es, bool backward)
 {
     SmallCall k;
-    return small_of(last, sh, es, backward, Map{}, Map{}, Map{}, k);
+    return small_of(last, sh, es, backward, Map{}, Map{}, Map{}, k) ? k.threads : 0;
 }
 
 int small_forward(bool last, int dtype, const Shape &sh, const Map &x, const Map &y, const Params &p, double *stats, hipStream_t st)

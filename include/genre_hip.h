@@ -459,7 +459,8 @@ int genre_render_bm_backward(const genre_tensor *grad_out, const genre_tensor *g
  * ws: fp64 scratch of at least genre_group_norm_workspace(x, groups, backward) values (-1: refused; 0: may be NULL), undefined
  * before and after; two calls that may run at once need two.  Sums and statistics are fp64 and added in a fixed order: equal inputs, equal bits.
  * No output may share memory with an input or another output.  The derivative of (leaky) ReLU at 0 is that of the negative side;
- * a ReLU that is off passes nothing on, whatever dy holds there.  N or S of zero: nothing but dw = db = 0 is written. */
+ * a ReLU that is off passes nothing on, whatever dy holds there.  N or S of zero: nothing but dw = db = 0 is written.
+ * Maps of 2^24 planes (N C) or more may be refused: a launch holds fewer than 2^32 threads. */
 int64_t genre_group_norm_workspace(const genre_tensor *x, int groups, int backward);
 
 int genre_group_norm_forward(const genre_tensor *x, const genre_tensor *y, const genre_tensor *weight, const genre_tensor *bias,

@@ -26,3 +26,20 @@ def test_sizes_that_no_map_has(lib, shape, stride, word):  # noqa: F811
     L, lib = lib
     for name, (rc, error) in entries(L, lib, desc(L, shape, stride=stride)).items():
         assert rc == 0 and word in error, (name, error)
+
+
+def test_more_threads_than_a_launch_holds(lib):  # noqa: F811
+    """workgroups times threads of 2^32 or more, in the one-workgroup form and in two passes: refused before any launch, and before
+    the caller allocates scratch"""
+    L, lib = lib
+    rows = lambda n: desc(L, (n, 8, 1), stride=(8, 1, 8))
+    for name, (rc, error) in entries(L, lib, rows(1 << 26), groups=1).items():
+        assert rc == 0 and b"too large for one launch" in error, (name, error)
+    assert lib.genre_group_norm_workspace(rows((1 << 26) - 1), C.c_int(1), C.c_int(0)) == 0
+    odd = lambda n: desc(L, (n, 4, 3), stride=(12, 3, 1))                  # (planes of an odd number of positions: the backward takes two passes)
+    got = entries(L, lib, odd(1 << 24), groups=1)
+    assert got["workspace"][0] == 1                                       # (0 values)
+    for name in ("backward workspace", "backward"):
+        rc, error = got[name]
+        assert rc == 0 and b"too large for one launch" in error, (name, error)
+    assert lib.genre_group_norm_workspace(odd((1 << 24) - 64), C.c_int(1), C.c_int(1)) > 0
