@@ -413,7 +413,10 @@ Tensor clip_grads(pybind11::handle tensors, double max_norm, int64_t kind, bool 
     const c10::DeviceGuard guard(l.device);
     const Tensor out = norm_and_factor("clip_grads_", l, kind, max_norm), norm = out.select(0, 0);
     if (error_if_nonfinite) {
-        const double v = norm.item<float>();
+        const double v = [&] {
+            pybind11::gil_scoped_release no_gil;                           // (this waits for the GPU: other threads go on)
+            return norm.item<float>();
+        }();
         TORCH_CHECK(std::isfinite(v), "clip_grads_: the norm of the gradients is ", v);
     }
     check_apart("clip_grads_", l);

@@ -42,6 +42,8 @@ def clip_grads_(tensors, max_norm, norm_type=2.0, error_if_nonfinite=False):
     A norm of infinity scales by 0 (infinities become NaN), NaN makes all NaN; error_if_nonfinite raises before anything is
     written instead, for which it waits for the GPU.  Tensors that share memory, or one that is listed twice, are refused."""
     kind, max_norm, tensors = _kind("clip_grads_", norm_type), _bound("clip_grads_", max_norm), _list(tensors)
+    if error_if_nonfinite:
+        tensors = tuple(tensors)                                          # (other threads run while it waits: the list stays what it was)
     return _native.clip_grads(tensors, max_norm, kind, error_if_nonfinite) if tensors else torch.tensor(0.0)
 
 
