@@ -6,7 +6,7 @@
 // grid twice on the DEFAULT stream; at batch 1 only 4 of its 512 blocks work.
 //
 // Here ONE launch covers both directions.  A workgroup owns 128 queries (two per
-// lane, riding in the two halves of packed-fp32 ops) and its waves each scan a
+// lane, which share the target loads and the loop) and its waves each scan a
 // different slice of the target cloud: 16 slices for a lone cloud pair, so that
 // 2048 x 2048 already puts a wave on every SIMD of 32 CUs; 8, 4 or 2 once the
 // batch alone fills the chip (longer scans per wave, less prologue and merge per
@@ -16,11 +16,12 @@
 // merged through LDS in slice order with a strict '<', which is exactly the
 // reference's "first minimum wins" (my_lib.c:20, nnd_cuda.cu:26,120).
 //
-// Issue cost on gfx950 (tools/valu_rate_bench.hip, tools/pk_f32_bench.hip): a
-// v_pk_{add,mul}_f32 takes ~4.2 cycles per wave for two pairs, a plain fp32 op on
-// VGPRs ~2.5 for one (4.2 with an SGPR operand), v_min_f32 / v_min3_f32 ~4.3.  The
-// scan is 4 packed ops + ~0.9 min + ~0.5 select per pair = ~22 cycles: a ceiling of
-// ~56 TFLOP/s for this un-fused 8-flop formulation (measured: 45 at 32 x 2048^2).
+// Issue cost on gfx950 (tools/valu_rate_bench.hip): a plain fp32 op takes ~2.5
+// cycles per wave on VGPRs and ~4.2 with an SGPR operand, v_min_f32 / v_min3_f32
+// ~4.3.  The scan is 3 subtractions from SGPRs + 5 ops + ~0.9 min + ~0.5 select per
+// pair = ~26 cycles: a ceiling of ~48 TFLOP/s for this un-fused 8-flop formulation
+// (measured: 48.0 at 32 x 2048^2).  Packed fp32 ops would serve two pairs in ~4.2
+// cycles (48.9 measured), but the library is built without them (Makefile).
 //
 // Distances use the reference's fp32 expression x*x + y*y + z*z evaluated left
 // to right WITHOUT fma contraction, so dist is bit-identical to the CPU
@@ -101,9 +102,8 @@ __global__ __launch_bounds__(kSlices * 64) void nnd_forward_kernel(int n, int m,
         for (int u = 0; u < kQ; u++) { best[u] = sqdist(qx[u], qy[u], qz[u], t[0], t[1], t[2]); bchunk[u] = k0; }
         int k = k0;
         const float *__restrict__ tp = t;
-        // main loop: the two queries of a lane ride in the two halves of packed fp32 ops (v_pk_add_f32 with a
-        // negated operand, v_pk_mul_f32: IEEE results identical to the scalar forms, 2 pairs per instruction)
-        static_assert(kQ == 2, "the packed main loop carries exactly two queries per lane");
+        // main loop: the two queries of a lane side by side
+        static_assert(kQ == 2, "the main loop carries exactly two queries per lane");
         const f2 px = {qx[0], qx[1]}, py = {qy[0], qy[1]}, pz = {qz[0], qz[1]};
         // the chunk after the current one is requested before the current one is evaluated: scalar loads return
         // out of order, so their only wait is "all outstanding" -- without the prefetch every iteration starts

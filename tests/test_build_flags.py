@@ -1,0 +1,14 @@
+"""How the library is compiled."""
+import os
+import subprocess
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "genre-shapehd_amd", "csrc")
+
+
+def test_no_source_is_compiled_with_packed_fp32():
+    lines = subprocess.run(["make", "-n", "-B", "-C", CSRC], capture_output=True, text=True, timeout=120, check=True).stdout.splitlines()
+    compiled = [line.split() for line in lines if ".hip -o " in line and " -c " in line]
+    assert {words[words.index("-c") + 1] for words in compiled} == {f for f in os.listdir(CSRC) if f.endswith(".hip")}
+    for words in compiled:
+        at = words.index("-packed-fp32-ops")
+        assert words[at - 3:at] == ["-Xclang", "-target-feature", "-Xclang"] and "-ffp-contract=off" in words

@@ -5,7 +5,7 @@
 set -e
 SRC="$1"; shift
 cd "$(dirname "$0")/../genre-shapehd_amd/csrc"
-FLAGS="-O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -fno-gpu-flush-denormals-to-zero -I../../include"
+FLAGS="-O3 -std=c++17 -fPIC -ffp-contract=off -fhip-fp32-correctly-rounded-divide-sqrt -fno-gpu-flush-denormals-to-zero -Xclang -target-feature -Xclang -packed-fp32-ops -I../../include"
 make -s
 mkdir -p ../../tools/variants
 OBJS=""
