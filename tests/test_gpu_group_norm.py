@@ -112,6 +112,7 @@ SHAPES = [
     (3, 20, 4, (5, 7, 3)), (2, 45, 5, (23, 17)), (1, 1, 1, (70, 3)), (1, 1023, 3, (3, 5)), (2, 1030, 2, (9,)), (1, 4104, 8, (2, 3)),
     (1, 16, 1, (1, 2, 3)), (9, 3, 3, (2,)), (2, 80, 8, (16, 15, 14)),
     # groups of more values than one workgroup holds (65536 forward, 32768 backward), of more channels, and at the border
+    # (the borders that the first kernels had; where they lie now, test_gpu_group_norm_borders.py has both sides of them)
     (2, 45, 1, (41, 40)), (1, 511, 1, (13, 11)), (1, 1030, 2, (9, 15)), (1, 1030, 1, (3,)), (1, 4104, 2, (5, 7)), (2, 7, 1, (101, 97)), (1, 3, 1, (40001,)),
     (1, 64, 2, (32, 32)), (1, 64, 2, (32, 33)), (1, 64, 1, (32, 32)), (1, 64, 1, (32, 33)), (1, 96, 1, (700,)),
     # more groups or channels than a second pass adds up itself; columns that run over a row's end; one channel

@@ -43,3 +43,25 @@ def test_more_threads_than_a_launch_holds(lib):  # noqa: F811
         rc, error = got[name]
         assert rc == 0 and b"too large for one launch" in error, (name, error)
     assert lib.genre_group_norm_workspace(odd((1 << 24) - 64), C.c_int(1), C.c_int(1)) > 0
+
+
+@pytest.mark.parametrize("dtype", (0, 2, 3), ids=("fp32", "bf16", "fp16"))
+def test_where_one_workgroup_ends(lib, dtype):  # noqa: F811
+    """a call of one image that takes the one-workgroup form needs no scratch"""
+    L, lib = lib
+
+    def one(cg, s, last, back):
+        d = desc(L, (1, 2 * cg, s), stride=(2 * cg * s, 1, 2 * cg) if last else (2 * cg * s, s, 1), dtype=dtype)
+        return lib.genre_group_norm_workspace(d, C.c_int(2), C.c_int(back)) == 0
+
+    for cg, s in ((1, 16384), (4, 4096), (64, 256), (1024, 16), (1023, 16)):
+        for last in (False, True):
+            assert one(cg, s, last, 0) and not one(cg, s + 1, last, 0), (cg, s, last)
+            assert not one(cg, s, last, 1)
+    for cg, s in ((1, 8192), (4, 2048), (64, 128), (512, 16)):
+        assert one(cg, s, True, 1) and not one(cg, s + 1, True, 1) and not one(cg, s, False, 1), (cg, s)
+    for cg, s in ((1, 4096), (4, 1024), (64, 64), (512, 8)):
+        assert one(cg, s, False, 1) and not one(cg, s + 4, False, 1), (cg, s)
+    for last in (False, True):
+        assert one(1024, 4, last, 0) and not one(1025, 4, last, 0)
+    assert not one(4, 1023, False, 1) and one(4, 1023, True, 1)            # (an odd number of positions: two passes backward)
