@@ -39,3 +39,27 @@ def test_function_transforms_are_refused(genre, dev):
                  lambda: torch.func.jvp(lambda t: genre.group_norm_act(t, 2, w), (x[0],), (x[0],))):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_a_refiner_with_group_norm_is_captured_and_replayed(genre, dev):
+    """as GenReInference(graph=True) does with the whole model: every replay is what the eager forward gives, to the convolutions' rounding"""
+    from genre_shapehd_amd.networks import Unet_3D
+    torch.manual_seed(2)
+    net = Unet_3D(norm="group").to(dev).eval()
+    x = torch.rand(1, 2, 128, 128, 128, device=dev)
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for _ in range(2):
+                net(x)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = net(x)
+        for _ in range(3):
+            x.uniform_()
+            want = net(x)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert (y - want).abs().max() <= 1e-4 * max(1.0, want.abs().max())
