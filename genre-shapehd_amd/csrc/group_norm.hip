@@ -18,7 +18,8 @@
 // where the second pass, which starts where the first ended, still finds x in the 256 MB cache.  Measured:
 //   4 x 20 x 64^3 fp32 channels last, leaky ReLU: forward 17 + 30 us (84 MB read, 84 MB read + 86 written), backward 28 + 42 us
 //   8 x 32 x 64^3 bf16 channels first, ReLU:      forward 22 + 42 us (134 MB,       134 + 134),            backward 41 + 61 us
-// y and dx are stored past the caches: a launch's end waits for what it left dirty in the L2s (58.7 -> 47.4 us and 88.8 -> 73.4).
+//   4 x 20 x 64^3 fp32 channels first, leaky ReLU: forward 15 + 27 us, backward 27 + 38 us;  8 x 32 x 64^3, ReLU: 41 + 84 and 85 + 137
+// y and dx are stored past the caches (group_norm.hpp).
 #include "group_norm.hpp"
 
 namespace genre {
