@@ -12,3 +12,10 @@ def test_no_source_is_compiled_with_packed_fp32():
     for words in compiled:
         at = words.index("-packed-fp32-ops")
         assert words[at - 3:at] == ["-Xclang", "-target-feature", "-Xclang"] and "-ffp-contract=off" in words
+
+
+def test_variants_of_the_library_hold_every_object():
+    """tools/build_variants.sh links one recompiled source with the other objects of the library"""
+    with open(os.path.join(CSRC, "..", "..", "tools", "build_variants.sh")) as f:
+        listed = next(line for line in f if line.startswith("for o in "))
+    assert {o + ".hip" for o in listed[len("for o in "):listed.index(";")].split()} == {f for f in os.listdir(CSRC) if f.endswith(".hip")}
