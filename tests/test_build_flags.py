@@ -19,3 +19,12 @@ def test_variants_of_the_library_hold_every_object():
     with open(os.path.join(CSRC, "..", "..", "tools", "build_variants.sh")) as f:
         listed = next(line for line in f if line.startswith("for o in "))
     assert {o + ".hip" for o in listed[len("for o in "):listed.index(";")].split()} == {f for f in os.listdir(CSRC) if f.endswith(".hip")}
+
+
+def test_build_compiles_whatever_is_built_already(genre, monkeypatch):
+    import __graft_entry__ as entry
+    calls = []
+    monkeypatch.setattr(subprocess, "check_call", calls.append)
+    monkeypatch.setattr(subprocess, "call", lambda *args, **kwargs: 3)
+    entry.build()
+    assert CSRC in calls[0] and all(words[0] == "make" and "-B" in words for words in calls)
